@@ -5,6 +5,9 @@ from .functional import (
     correlation,
     unsup_loss_scale,
     endpoint_error_sum,
+    draw_rng,
+    dropout,
+    group_norm,
     hip_available,
     require_hip,
 )
@@ -16,6 +19,9 @@ __all__ = [
     "correlation",
     "unsup_loss_scale",
     "endpoint_error_sum",
+    "draw_rng",
+    "dropout",
+    "group_norm",
     "hip_available",
     "require_hip",
 ]

@@ -225,3 +225,188 @@ def endpoint_error_sum(flow: torch.Tensor, flow_gt: torch.Tensor) -> torch.Tenso
                                      flow_gt.contiguous().float())
     d = (flow.float() - flow_gt.float())
     return torch.sqrt(d[:, 0] ** 2 + d[:, 1] ** 2).sum()
+
+
+# ---------------------------------------------------------------------------
+# dropout from a counter-based generator; group norm + activation + dropout
+# ---------------------------------------------------------------------------
+_ACT_CODES = {None: 0, "none": 0, "elu": 1, "leaky_relu": 2, "relu": 3,
+              "silu": 4}
+_MAX_GROUPS = 4096  # the kernels hold a sample's group statistics in LDS
+
+
+def draw_rng(device, generator: torch.Generator | None = None) -> torch.Tensor:
+    """A fresh (seed, offset) for `dropout` and `group_norm`: two int64 drawn
+    from torch's generator of `device`, and left there.
+
+    Follows torch.manual_seed, a saved and restored generator state
+    (activation recomputation) and graph capture: every replay draws anew.
+    """
+    return torch.randint(0, 2**63 - 1, (2,), device=device,
+                         generator=generator)
+
+
+def _check_act(act):
+    if act not in _ACT_CODES:
+        raise ValueError(f"unknown activation {act!r}")
+
+
+def _check_float(x, name):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name}: a tensor expected, got {type(x).__name__}")
+    allowed = (torch.float32, torch.float16, torch.bfloat16)
+    if x.dtype not in allowed and (x.is_cuda or x.dtype != torch.float64):
+        raise TypeError(f"{name}: float32, float16 or bfloat16 expected, got "
+                        f"{x.dtype}")
+
+
+def _check_dropout(p, rng, x):
+    """-> (p, rng tensor or None, seed, offset)"""
+    if isinstance(p, bool) or not isinstance(p, (int, float)):
+        raise TypeError(f"dropout probability: a number expected, got {p!r}")
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout probability must lie in [0, 1], got {p}")
+    if p == 0.0:
+        return p, None, 0, 0
+    if rng is None:
+        return p, draw_rng(x.device), 0, 0
+    if isinstance(rng, torch.Tensor):
+        if rng.dtype != torch.int64 or rng.shape != (2,):
+            raise ValueError("rng: an int64 tensor [seed, offset] expected, "
+                             f"got {rng.dtype} {tuple(rng.shape)}")
+        if rng.device != x.device:
+            raise ValueError(f"rng is on {rng.device}, the input on {x.device}")
+        return p, rng.contiguous(), 0, 0
+    if (isinstance(rng, (tuple, list)) and len(rng) == 2
+            and all(isinstance(v, int) and not isinstance(v, bool)
+                    for v in rng)):
+        if not all(0 <= v < 2**63 for v in rng):
+            raise ValueError(f"rng: seed and offset lie in [0, 2^63), got {rng}")
+        return p, None, rng[0], rng[1]
+    raise TypeError("rng: an int64 tensor of 2 or a pair of ints expected, got "
+                    f"{rng!r}")
+
+
+def _rng_tensor(rng, seed, offset):
+    return torch.tensor([seed, offset]) if rng is None else rng
+
+
+def _dense_format(x):
+    if (x.dim() == 4 and not x.is_contiguous()
+            and x.is_contiguous(memory_format=torch.channels_last)):
+        return torch.channels_last
+    return torch.contiguous_format
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, rng, seed, offset, act):
+        ctx.save_for_backward(x if act else None, rng)
+        ctx.meta = (p, seed, offset, act, _dense_format(x))
+        return require_hip().dropout_forward(x, act, p, rng, seed, offset)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, rng = ctx.saved_tensors
+        p, seed, offset, act, fmt = ctx.meta
+        gx = require_hip().dropout_backward(
+            gy.contiguous(memory_format=fmt), x, act, p, rng, seed, offset)
+        return gx, None, None, None, None, None
+
+
+def dropout(x: torch.Tensor, p: float = 0.5, rng=None,
+            act: str | None = None) -> torch.Tensor:
+    """act(x) / (1 - p) where kept, 0 where dropped (with probability p).
+
+    x: float32, float16 or bfloat16, any shape.  rng: what the mask is a
+    function of, an int64 tensor [seed, offset] on x's device or a pair of
+    ints in [0, 2^63); None draws one (`draw_rng`).  The mask is computed from
+    (seed, offset, element) by Philox4x32-10 in both directions and never
+    stored; elements are counted in memory order, channels fastest in
+    channels-last tensors, and tensors of other strides are made contiguous.
+    p is held to 2^-32.  A captured graph replays the mask of a pair of ints;
+    it reads a tensor anew, and draws anew where rng is None.
+    """
+    _check_float(x, "dropout")
+    _check_act(act)
+    p, rng, seed, offset = _check_dropout(p, rng, x)
+    x = x.contiguous(memory_format=_dense_format(x))
+    if not x.is_cuda:
+        return ref.dropout(x, p, _rng_tensor(rng, seed, offset), act)
+    code = _ACT_CODES[act]
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Dropout.apply(x, p, rng, seed, offset, code)
+    return require_hip().dropout_forward(x, code, p, rng, seed, offset)
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act, p, rng, seed, offset):
+        y, mean, rstd = require_hip().group_norm_forward(
+            x, groups, weight, bias, eps, act, p, rng, seed, offset)
+        ctx.save_for_backward(x, weight, bias, mean, rstd, rng)
+        ctx.meta = (act, p, seed, offset)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, weight, bias, mean, rstd, rng = ctx.saved_tensors
+        act, p, seed, offset = ctx.meta
+        gx, gw, gb = require_hip().group_norm_backward(
+            gy.contiguous(memory_format=torch.channels_last), x, weight, bias,
+            mean, rstd, act, p, rng, seed, offset, *ctx.needs_input_grad[:3])
+        return (gx, gw, gb) + (None,) * 7
+
+
+def group_norm(x: torch.Tensor, num_groups: int,
+               weight: torch.Tensor | None = None,
+               bias: torch.Tensor | None = None, eps: float = 1e-5,
+               act: str | None = None, dropout: float = 0.0,
+               rng=None) -> torch.Tensor:
+    """Group norm, affine, activation and dropout of [B, C, H, W] in one go.
+
+    x: float32, float16 or bfloat16; the result is channels last, and an x
+    that is not is copied.  Statistics and all arithmetic are fp32.  act: None,
+    "elu", "leaky_relu" (0.1), "relu" or "silu".  dropout: its probability;
+    rng as for `dropout`, whose mask for the same rng is the same.
+    """
+    _check_float(x, "group_norm")
+    if x.dim() != 4:
+        raise ValueError(f"group_norm: [B, C, H, W] expected, got "
+                         f"{tuple(x.shape)}")
+    c = x.shape[1]
+    if isinstance(num_groups, bool) or not isinstance(num_groups, int):
+        raise TypeError(f"group_norm: num_groups must be an int, got "
+                        f"{num_groups!r}")
+    if not 1 <= num_groups <= _MAX_GROUPS or c == 0 or c % num_groups:
+        raise ValueError(f"group_norm: {c} channels in {num_groups} groups "
+                         f"(at most {_MAX_GROUPS})")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        _check_float(t, f"group_norm {name}")
+        if t.shape != (c,) or t.device != x.device:
+            raise ValueError(f"group_norm: {name} must be [{c}] on {x.device}, "
+                             f"got {tuple(t.shape)} on {t.device}")
+    if not (eps > 0.0 and eps < float("inf")):
+        raise ValueError(f"group_norm: eps must be positive, got {eps}")
+    _check_act(act)
+    p, rng, seed, offset = _check_dropout(dropout, rng, x)
+    x = x.contiguous(memory_format=torch.channels_last)
+    if not x.is_cuda:
+        y = ref.group_norm(x, num_groups, weight, bias, eps, act, p,
+                           _rng_tensor(rng, seed, offset) if p else None)
+        return y.contiguous(memory_format=torch.channels_last)
+    # the kernels read fp32 parameters; a cast is part of the graph
+    weight = None if weight is None else weight.float().contiguous()
+    bias = None if bias is None else bias.float().contiguous()
+    code = _ACT_CODES[act]
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _GroupNorm.apply(x, weight, bias, num_groups, eps, code, p, rng,
+                                seed, offset)
+    return require_hip().group_norm_forward(
+        x, num_groups, weight, bias, eps, code, p, rng, seed, offset)[0]

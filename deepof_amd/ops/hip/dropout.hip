@@ -1,0 +1,148 @@
+// Activation + dropout with a mask that is never stored, for gfx950.
+//
+//   forward   y  = kept(i) ? act(x_i) / (1 - p) : 0
+//   backward  dx = kept(i) ? gy_i / (1 - p) * act'(x_i) : 0
+//
+// kept(i) is computed from (seed, offset, i) in both directions
+// (philox.hip.h), so neither a mask is written nor read back.
+
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPException.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/extension.h>
+
+#include "dropout_args.h"
+#include "philox.hip.h"
+#include "vec.hip.h"
+
+namespace {
+
+constexpr int BLOCK = 256;
+constexpr int UNROLL = 4;  // vectors of 8 in flight per thread
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load8(const T* at, int count, float (&v)[8]) {
+  if (WIDE && count == 8) {
+    unpack<T, 8>(load_pack<T, 8>(at), v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = k < count ? (float)at[k] : 0.0f;
+  }
+}
+
+// WIDE: every pointer is aligned to 16 bytes.  gy is null going forwards; x
+// is null where nothing of it is needed (backwards without an activation).
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(BLOCK) void dropout_kernel(
+    const T* __restrict__ x, const T* __restrict__ gy, T* __restrict__ out,
+    int64_t n, int act, DropoutArgs d) {
+  const DropoutState st = dropout_state(d);
+  const int64_t first = (int64_t)blockIdx.x * (BLOCK * UNROLL) + threadIdx.x;
+  float v[UNROLL][8], z[UNROLL][8];
+#pragma unroll
+  for (int i = 0; i < UNROLL; ++i) {
+    const int64_t at = (first + i * BLOCK) * 8;
+    const int count = (int)min((int64_t)8, n - at);
+    if (count <= 0) continue;
+    if (x) load8<T, WIDE>(x + at, count, z[i]);
+    if (gy) load8<T, WIDE>(gy + at, count, v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < UNROLL; ++i) {
+    const int64_t j = first + i * BLOCK;
+    const int64_t at = j * 8;
+    const int count = (int)min((int64_t)8, n - at);
+    if (count <= 0) continue;
+    if (gy) {
+      if (x) act_backward<8>(act, z[i], v[i]);
+    } else {
+      act_apply<T, 8>(act, z[i]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[i][k] = z[i][k];
+    }
+    if (d.on) dropout_apply<8>(d, st, (uint64_t)at, v[i]);
+    if (WIDE && count == 8) {
+      store_pack<T, 8>(out + at, pack<T, 8>(v[i]));
+    } else {
+      for (int k = 0; k < count; ++k) out[at + k] = (T)v[i][k];
+    }
+  }
+}
+
+bool wide(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename T>
+void launch(const void* x, const void* gy, void* out, int64_t n, int act,
+            const DropoutArgs& d) {
+  const int64_t per_block = (int64_t)BLOCK * UNROLL * 8;
+  const int64_t blocks = (n + per_block - 1) / per_block;
+  TORCH_CHECK(blocks < (1ll << 31), "dropout: tensor too large");
+  const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
+  const bool w = wide(x) && wide(gy) && wide(out);
+  if (w)
+    dropout_kernel<T, true><<<(unsigned)blocks, BLOCK, 0, stream>>>(
+        (const T*)x, (const T*)gy, (T*)out, n, act, d);
+  else
+    dropout_kernel<T, false><<<(unsigned)blocks, BLOCK, 0, stream>>>(
+        (const T*)x, (const T*)gy, (T*)out, n, act, d);
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+}
+
+at::Tensor dropout_any(const at::Tensor& like, const void* x, const void* gy,
+                       long act, const DropoutArgs& d) {
+  auto out = at::empty_like(like);  // dense input: the same strides
+  const int64_t n = like.numel();
+  if (n == 0) return out;
+  switch (like.scalar_type()) {
+    case at::kFloat:
+      launch<float>(x, gy, out.data_ptr(), n, (int)act, d);
+      break;
+    case at::kHalf:
+      launch<fp16_t>(x, gy, out.data_ptr(), n, (int)act, d);
+      break;
+    case at::kBFloat16:
+      launch<bf16_t>(x, gy, out.data_ptr(), n, (int)act, d);
+      break;
+    default:
+      TORCH_CHECK(false, "dropout: float32, float16 or bfloat16 expected");
+  }
+  return out;
+}
+
+void check_dense(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), "dropout: ", name, " must be on the GPU");
+  TORCH_CHECK(t.is_contiguous() ||
+                  t.is_contiguous(at::MemoryFormat::ChannelsLast),
+              "dropout: ", name, " must be contiguous or channels last");
+}
+
+}  // namespace
+
+at::Tensor dropout_forward(at::Tensor x, long act, double p,
+                           c10::optional<at::Tensor> rng, int64_t seed,
+                           int64_t offset) {
+  check_dense(x, "x");
+  c10::DeviceGuard guard(x.device());
+  return dropout_any(x, x.data_ptr(), nullptr, act,
+                     dropout_args(p, rng, seed, offset, x));
+}
+
+at::Tensor dropout_backward(at::Tensor gy, c10::optional<at::Tensor> x,
+                            long act, double p, c10::optional<at::Tensor> rng,
+                            int64_t seed, int64_t offset) {
+  check_dense(gy, "gy");
+  c10::DeviceGuard guard(gy.device());
+  const void* xp = nullptr;
+  if (act != ACT_NONE) {
+    const auto cl = at::MemoryFormat::ChannelsLast;
+    TORCH_CHECK(x.has_value() && x->sizes() == gy.sizes() &&
+                    ((x->is_contiguous() && gy.is_contiguous()) ||
+                     (x->is_contiguous(cl) && gy.is_contiguous(cl))) &&
+                    x->scalar_type() == gy.scalar_type() &&
+                    x->device() == gy.device(),
+                "dropout: x must be like gy");
+    xp = x->data_ptr();
+  }
+  return dropout_any(gy, xp, gy.data_ptr(), act,
+                     dropout_args(p, rng, seed, offset, gy));
+}

@@ -368,3 +368,110 @@ def unsup_loss_scale_edge_aware(
     total = photo + lambda_smooth * (u_loss + v_loss)
     return {"total": total, "photo": photo, "u_loss": u_loss,
             "v_loss": v_loss}
+
+
+# ---------------------------------------------------------------------------
+# Activations, dropout from a counter-based generator, group norm
+# ---------------------------------------------------------------------------
+def activation(z: torch.Tensor, act: str | None) -> torch.Tensor:
+    if act in (None, "none"):
+        return z
+    if act == "elu":
+        return F.elu(z)
+    if act == "leaky_relu":
+        return F.leaky_relu(z, 0.1)
+    if act == "relu":
+        return F.relu(z)
+    if act == "silu":
+        return F.silu(z)
+    raise ValueError(f"unknown activation {act!r}")
+
+
+def philox4x32(counter, key) -> list[torch.Tensor]:
+    """Philox4x32-10 (Salmon, Moraes, Dror, Shaw, "Parallel random numbers:
+    as easy as 1, 2, 3", SC 2011): four 32-bit words from a counter of four
+    and a key of two, each an int64 tensor of 32-bit values."""
+    mask = 0xFFFFFFFF
+    c0, c1, c2, c3 = counter
+    k0, k1 = key
+    for _ in range(10):
+        a, b = c0 * 0xD2511F53, c2 * 0xCD9E8D57  # mod 2^64: all that is used
+        c0, c1, c2, c3 = (((b >> 32) & mask) ^ c1 ^ k0, b & mask,
+                          ((a >> 32) & mask) ^ c3 ^ k1, a & mask)
+        k0, k1 = (k0 + 0x9E3779B9) & mask, (k1 + 0xBB67AE85) & mask
+    return [c0, c1, c2, c3]
+
+
+def dropout_numbers(n: int, rng: torch.Tensor) -> torch.Tensor:
+    """u(i) in [0, 2^32) for i < n: element i is dropped iff
+    u(i) < round(p * 2^32).
+
+    With j = i // 8 and s = i % 8, the upper 16 bits of u(i) are the s-th 16
+    bits (each word's low half first) of Philox4x32-10 for the key rng[0] and
+    the counter (j, rng[1]); its lower 16 bits are the same for the counter
+    (j + 2^63, rng[1]).
+    """
+    mask = 0xFFFFFFFF
+    seed, offset = rng[0], rng[1]
+    j = torch.arange((n + 7) // 8, device=rng.device)
+    key = (seed & mask, (seed >> 32) & mask)
+    rest = (offset & mask, (offset >> 32) & mask)
+
+    def halves(tag):
+        words = philox4x32((j & mask, (j >> 32) | tag) + rest, key)
+        return torch.stack([w >> s & 0xFFFF for w in words for s in (0, 16)],
+                           dim=1).reshape(-1)[:n]
+
+    return (halves(0) << 16) | halves(1 << 31)
+
+
+def dropout_keep(like: torch.Tensor, p: float,
+                 rng: torch.Tensor) -> torch.Tensor:
+    """Which elements of `like` are kept; elements are counted in memory
+    order, channels fastest if `like` is channels last."""
+    u = dropout_numbers(like.numel(), rng)
+    keep = u >= math.floor(p * 2**32 + 0.5)
+    if like.dim() == 4 and not like.is_contiguous() \
+            and like.is_contiguous(memory_format=torch.channels_last):
+        b, c, h, w = like.shape
+        return keep.reshape(b, h, w, c).permute(0, 3, 1, 2)
+    return keep.reshape(like.shape)
+
+
+def dropout(x: torch.Tensor, p: float, rng: torch.Tensor,
+            act: str | None = None) -> torch.Tensor:
+    """act(x) / (1 - p) where kept, 0 elsewhere."""
+    wide = x if x.dtype == torch.float64 else x.float()
+    if p == 0:
+        return activation(wide, act).to(x.dtype)
+    keep = dropout_keep(x, p, rng)
+    scale = 1.0 / (1.0 - p) if p < 1 else 0.0
+    # in front of act too, so that NaN in dropped places has no gradient
+    y = activation(torch.where(keep, wide, 0.0), act)
+    return torch.where(keep, y * scale, 0.0).to(x.dtype)
+
+
+def group_norm(x: torch.Tensor, num_groups: int, weight=None, bias=None,
+               eps: float = 1e-5, act: str | None = None, p: float = 0.0,
+               rng: torch.Tensor | None = None) -> torch.Tensor:
+    """Group norm + activation + dropout of channels-last [B, C, H, W]."""
+    b, c, h, w = x.shape
+    if x.numel() == 0:  # in the graph all the same: its gradients are zeros
+        y = x * 1.0
+        for t in (weight, bias):
+            y = y if t is None else y + t.to(x.dtype).view(1, -1, 1, 1)
+        return y
+    wide = x if x.dtype == torch.float64 else x.float()
+    v = wide.permute(0, 2, 3, 1).reshape(b, h * w, num_groups, -1)
+    centred = v - v.mean((1, 3), keepdim=True)
+    var = (centred * centred).mean((1, 3), keepdim=True)
+    z = (centred * torch.rsqrt(var + eps)).reshape(b, h, w, c)
+    if weight is not None:
+        z = z * weight.to(z.dtype)
+    if bias is not None:
+        z = z + bias.to(z.dtype)
+    y = activation(z.permute(0, 3, 1, 2), act)
+    if p > 0:
+        scale = 1.0 / (1.0 - p) if p < 1 else 0.0
+        y = torch.where(dropout_keep(x, p, rng), y * scale, 0.0)
+    return y.to(x.dtype)

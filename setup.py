@@ -25,6 +25,8 @@ ext = CUDAExtension(
         os.path.join(SRC, "adam.hip"),
         os.path.join(SRC, "conv_mfma.hip"),
         os.path.join(SRC, "conv_wrw2.hip"),
+        os.path.join(SRC, "group_norm.hip"),
+        os.path.join(SRC, "dropout.hip"),
     ],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
