@@ -18,74 +18,95 @@
 namespace {
 
 constexpr int BLOCK = 256;
-constexpr int UNROLL = 4;  // vectors of 8 in flight per thread
+constexpr int UNROLL = 2;  // vectors of 8 in flight per thread
 
 template <typename T, bool WIDE>
-__device__ __forceinline__ void load8(const T* at, int count, float (&v)[8]) {
-  if (WIDE && count == 8) {
-    unpack<T, 8>(load_pack<T, 8>(at), v);
-  } else {
+__device__ __forceinline__ Pack<T, 8> load8(const T* at, int count) {
+  if (WIDE && count == 8) return load_pack<T, 8>(at);
+  Pack<T, 8> p;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = k < count ? (float)at[k] : 0.0f;
-  }
+  for (int k = 0; k < 8; ++k) p.v[k] = k < count ? at[k] : (T)0.0f;
+  return p;
 }
 
-// WIDE: every pointer is aligned to 16 bytes.  gy is null going forwards; x
-// is null where nothing of it is needed (backwards without an activation).
-template <typename T, bool WIDE>
+// WIDE: every pointer is aligned to 16 bytes.  Forwards reads x alone;
+// backwards gy, and x where the activation has a slope.
+template <typename T, bool WIDE, bool BACK, int ACT>
 __global__ __launch_bounds__(BLOCK) void dropout_kernel(
     const T* __restrict__ x, const T* __restrict__ gy, T* __restrict__ out,
     int64_t n, int act, DropoutArgs d) {
+  const bool need_x = !BACK || (ACT == ACT_ANY ? act : ACT) != ACT_NONE;
   const DropoutState st = dropout_state(d);
   const int64_t first = (int64_t)blockIdx.x * (BLOCK * UNROLL) + threadIdx.x;
-  float v[UNROLL][8], z[UNROLL][8];
+  Pack<T, 8> rx[UNROLL], rg[UNROLL];
 #pragma unroll
   for (int i = 0; i < UNROLL; ++i) {
     const int64_t at = (first + i * BLOCK) * 8;
     const int count = (int)min((int64_t)8, n - at);
     if (count <= 0) continue;
-    if (x) load8<T, WIDE>(x + at, count, z[i]);
-    if (gy) load8<T, WIDE>(gy + at, count, v[i]);
+    if (need_x) rx[i] = load8<T, WIDE>(x + at, count);
+    if (BACK) rg[i] = load8<T, WIDE>(gy + at, count);
   }
 #pragma unroll
   for (int i = 0; i < UNROLL; ++i) {
-    const int64_t j = first + i * BLOCK;
-    const int64_t at = j * 8;
+    const int64_t at = (first + i * BLOCK) * 8;
     const int count = (int)min((int64_t)8, n - at);
     if (count <= 0) continue;
-    if (gy) {
-      if (x) act_backward<8>(act, z[i], v[i]);
+    float v[8];
+    if (BACK) {
+      unpack<T, 8>(rg[i], v);
+      if (need_x) {
+        float z[8];
+        unpack<T, 8>(rx[i], z);
+        act_backward<ACT, 8>(act, z, v);
+      }
     } else {
-      act_apply<T, 8>(act, z[i]);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[i][k] = z[i][k];
+      unpack<T, 8>(rx[i], v);
+      act_apply<T, ACT, 8>(act, v);
     }
-    if (d.on) dropout_apply<8>(d, st, (uint64_t)at, v[i]);
+    if (d.on) dropout_apply<8>(d, st, (uint64_t)at, v);
+    const Pack<T, 8> o = pack<T, 8>(v);
     if (WIDE && count == 8) {
-      store_pack<T, 8>(out + at, pack<T, 8>(v[i]));
+      store_pack<T, 8>(out + at, o);
     } else {
-      for (int k = 0; k < count; ++k) out[at + k] = (T)v[i][k];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < count) out[at + k] = o.v[k];
     }
   }
 }
 
 bool wide(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <typename T>
+template <typename T, bool BACK>
 void launch(const void* x, const void* gy, void* out, int64_t n, int act,
             const DropoutArgs& d) {
   const int64_t per_block = (int64_t)BLOCK * UNROLL * 8;
   const int64_t blocks = (n + per_block - 1) / per_block;
   TORCH_CHECK(blocks < (1ll << 31), "dropout: tensor too large");
   const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
-  const bool w = wide(x) && wide(gy) && wide(out);
-  if (w)
-    dropout_kernel<T, true><<<(unsigned)blocks, BLOCK, 0, stream>>>(
-        (const T*)x, (const T*)gy, (T*)out, n, act, d);
-  else
-    dropout_kernel<T, false><<<(unsigned)blocks, BLOCK, 0, stream>>>(
-        (const T*)x, (const T*)gy, (T*)out, n, act, d);
+  auto kernel = dropout_kernel<T, false, BACK, ACT_ANY>;
+  if (wide(x) && wide(gy) && wide(out)) {
+    switch (act) {
+      case ACT_ELU: kernel = dropout_kernel<T, true, BACK, ACT_ELU>; break;
+      case ACT_LEAKY: kernel = dropout_kernel<T, true, BACK, ACT_LEAKY>; break;
+      case ACT_RELU: kernel = dropout_kernel<T, true, BACK, ACT_RELU>; break;
+      case ACT_SILU: kernel = dropout_kernel<T, true, BACK, ACT_SILU>; break;
+      default: kernel = dropout_kernel<T, true, BACK, ACT_NONE>; break;
+    }
+  }
+  kernel<<<(unsigned)blocks, BLOCK, 0, stream>>>(
+      (const T*)x, (const T*)gy, (T*)out, n, act, d);
   C10_HIP_KERNEL_LAUNCH_CHECK();
+}
+
+template <typename T>
+void launch_any(const void* x, const void* gy, void* out, int64_t n, int act,
+                const DropoutArgs& d) {
+  if (gy)
+    launch<T, true>(x, gy, out, n, act, d);
+  else
+    launch<T, false>(x, nullptr, out, n, act, d);
 }
 
 at::Tensor dropout_any(const at::Tensor& like, const void* x, const void* gy,
@@ -95,13 +116,13 @@ at::Tensor dropout_any(const at::Tensor& like, const void* x, const void* gy,
   if (n == 0) return out;
   switch (like.scalar_type()) {
     case at::kFloat:
-      launch<float>(x, gy, out.data_ptr(), n, (int)act, d);
+      launch_any<float>(x, gy, out.data_ptr(), n, (int)act, d);
       break;
     case at::kHalf:
-      launch<fp16_t>(x, gy, out.data_ptr(), n, (int)act, d);
+      launch_any<fp16_t>(x, gy, out.data_ptr(), n, (int)act, d);
       break;
     case at::kBFloat16:
-      launch<bf16_t>(x, gy, out.data_ptr(), n, (int)act, d);
+      launch_any<bf16_t>(x, gy, out.data_ptr(), n, (int)act, d);
       break;
     default:
       TORCH_CHECK(false, "dropout: float32, float16 or bfloat16 expected");

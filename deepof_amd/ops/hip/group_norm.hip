@@ -38,7 +38,7 @@ namespace {
 
 constexpr int WAVE = 64;
 constexpr int BLOCK = 256;       // threads of the split route's blocks
-constexpr int UNROLL = 4;        // vectors in flight per thread and tensor
+constexpr int UNROLL = 2;        // vectors in flight per thread and tensor
 constexpr int MAX_GROUPS = 4096; // their statistics live in LDS
 
 struct Shape {
@@ -52,10 +52,16 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
-// Pixels [first, last) of split s of n.
-__device__ __forceinline__ int64_t split_at(int64_t hw, int s, int n) {
-  return hw * s / n;
-}
+// Pixels cut into n pieces, the first `more` of them one longer than `size`.
+struct Cut {
+  int n, size, more;
+  __device__ __forceinline__ int first(int i) const {
+    return i * size + min(i, more);
+  }
+  __device__ __forceinline__ int pixels(int i) const {
+    return size + (i < more ? 1 : 0);
+  }
+};
 
 // Joins the (n, mean, M2) of entries into lane-uniform totals, each lane
 // bringing one entry at a time through `get(i, n, mean, m2)`.  Two passes:
@@ -104,14 +110,13 @@ __device__ __forceinline__ float rstd_of(float m2, float n, float eps) {
 template <typename T, int V, bool ONE>
 __global__ __launch_bounds__(BLOCK) void gn_stats(const T* __restrict__ x,
                                                   float2* __restrict__ part,
-                                                  Shape s, int splits) {
+                                                  Shape s, Cut cut) {
   constexpr int A = ONE ? 1 : V;
   __shared__ float2 red[BLOCK * A];
   extern __shared__ float joined[];  // [3][g]: n, mean, M2 so far
-  const int split = blockIdx.x % splits, b = blockIdx.x / splits;
-  const int64_t p0 = split_at(s.hw, split, splits);
-  const int pixels = (int)(split_at(s.hw, split + 1, splits) - p0);
-  const T* base = x + ((int64_t)b * s.hw + p0) * s.c;
+  const int split = blockIdx.x % cut.n, b = blockIdx.x / cut.n;
+  const int pixels = cut.pixels(split);
+  const T* base = x + ((int64_t)b * s.hw + cut.first(split)) * s.c;
   const int nv = s.c / V;                // columns of V channels
   const int unit = V / A;                // channels per entry
   const int upg = s.cg / unit;           // entries per group and row
@@ -201,29 +206,28 @@ __global__ __launch_bounds__(BLOCK) void gn_stats(const T* __restrict__ x,
     __syncthreads();
   }
   for (int g = threadIdx.x; g < s.g; g += BLOCK)
-    part[((int64_t)b * s.g + g) * splits + split] =
+    part[((int64_t)b * s.g + g) * cut.n + split] =
         make_float2(joined[s.g + g], joined[2 * s.g + g]);
 }
 
 // Block (chunk, sample): joins the sample's partial statistics, then reads x
 // and writes y.  The first block of a sample leaves its mean and rstd.
-template <typename T, int V>
+template <typename T, int V, int ACT>
 __global__ __launch_bounds__(BLOCK) void gn_apply(
     const T* __restrict__ x, T* __restrict__ y, const float* __restrict__ w,
     const float* __restrict__ bias, const float2* __restrict__ part,
     float* __restrict__ mean_out, float* __restrict__ rstd_out, Shape s,
-    int splits, int chunks, float eps, int act, DropoutArgs d) {
+    Cut cut, Cut chunks, float eps, int act, DropoutArgs d) {
   extern __shared__ float stat[];  // [2][g]: mean, rstd
-  const int chunk = blockIdx.x % chunks, b = blockIdx.x / chunks;
+  const int chunk = blockIdx.x % chunks.n, b = blockIdx.x / chunks.n;
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
   const DropoutState st = dropout_state(d);
   for (int g = wave; g < s.g; g += BLOCK / WAVE) {
-    const float2* e = part + ((int64_t)b * s.g + g) * splits;
+    const float2* e = part + ((int64_t)b * s.g + g) * cut.n;
     float n, mean, m2;
-    join(splits, lane,
+    join(cut.n, lane,
          [&](int i, float& ni, float& mi, float& qi) {
-           ni = (float)(split_at(s.hw, i + 1, splits) -
-                        split_at(s.hw, i, splits)) * (float)s.cg;
+           ni = (float)cut.pixels(i) * (float)s.cg;
            mi = e[i].x;
            qi = e[i].y;
          },
@@ -239,9 +243,8 @@ __global__ __launch_bounds__(BLOCK) void gn_apply(
     }
   }
   __syncthreads();
-  const int64_t p0 = split_at(s.hw, chunk, chunks);
-  const int pixels = (int)(split_at(s.hw, chunk + 1, chunks) - p0);
-  const int64_t from = ((int64_t)b * s.hw + p0) * s.c;
+  const int pixels = chunks.pixels(chunk);
+  const int64_t from = ((int64_t)b * s.hw + chunks.first(chunk)) * s.c;
   const int nv = s.c / V;
   for (int c0 = 0; c0 < nv; c0 += BLOCK) {
     const int cols = min(BLOCK, nv - c0);
@@ -263,7 +266,7 @@ __global__ __launch_bounds__(BLOCK) void gn_apply(
       const int64_t at = from + (int64_t)p * s.c + ch;
 #pragma unroll
       for (int j = 0; j < V; ++j) v[j] = fmaf(v[j] - m[j], a[j], o[j]);
-      act_apply<T, V>(act, v);
+      act_apply<T, ACT, V>(act, v);
       if (d.on) dropout_apply<V>(d, st, (uint64_t)at, v);
       store_pack<T, V>(y + at, pack<T, V>(v));
     };
@@ -304,7 +307,7 @@ __device__ __forceinline__ void load_channel(Channel<V>& k, int ch, int cg,
 }
 
 // (x, gy) -> (xhat, gz)
-template <int V>
+template <int ACT, int V>
 __device__ __forceinline__ void through(const Channel<V>& k, int act,
                                         const DropoutArgs& d,
                                         const DropoutState& st, uint64_t at,
@@ -316,30 +319,29 @@ __device__ __forceinline__ void through(const Channel<V>& k, int act,
     x[j] = (x[j] - k.mean[j]) * k.rstd[j];
     z[j] = fmaf(x[j], k.w[j], k.b[j]);
   }
-  act_backward<V>(act, z, g);
+  act_backward<ACT, V>(act, z, g);
 }
 
 // Block (split, sample): sums of gz and gz xhat of every channel over the
 // split's pixels.  part_c: [2][b * splits][c]; part_g: [b][g][splits] of the
 // same sums weighted by w and joined over the group.
-template <typename T, int V>
+template <typename T, int V, int ACT>
 __global__ __launch_bounds__(BLOCK) void gn_bwd_sums(
     const T* __restrict__ x, const T* __restrict__ gy,
     const float* __restrict__ w, const float* __restrict__ bias,
     const float* __restrict__ mean, const float* __restrict__ rstd,
     float* __restrict__ part_c, float2* __restrict__ part_g, Shape s,
-    int splits, int act, DropoutArgs d) {
+    Cut cut, int act, DropoutArgs d) {
   __shared__ float red[2][BLOCK * V];
   extern __shared__ float joined[];  // [2][g]
-  const int split = blockIdx.x % splits, b = blockIdx.x / splits;
+  const int split = blockIdx.x % cut.n, b = blockIdx.x / cut.n;
   const DropoutState st = dropout_state(d);
-  const int64_t p0 = split_at(s.hw, split, splits);
-  const int pixels = (int)(split_at(s.hw, split + 1, splits) - p0);
-  const int64_t from = ((int64_t)b * s.hw + p0) * s.c;
+  const int pixels = cut.pixels(split);
+  const int64_t from = ((int64_t)b * s.hw + cut.first(split)) * s.c;
   const int nv = s.c / V;
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
-  float* out1 = part_c + ((int64_t)b * splits + split) * s.c;
-  float* out2 = out1 + (int64_t)s.b * splits * s.c;
+  float* out1 = part_c + ((int64_t)b * cut.n + split) * s.c;
+  float* out2 = out1 + (int64_t)s.b * cut.n * s.c;
   mean += (int64_t)b * s.g;
   rstd += (int64_t)b * s.g;
 
@@ -358,7 +360,7 @@ __global__ __launch_bounds__(BLOCK) void gn_bwd_sums(
         float h[V], g[V];
         unpack<T, V>(rx, h);
         unpack<T, V>(rg, g);
-        through<V>(k, act, d, st, (uint64_t)(from + (int64_t)p * s.c + ch), h,
+        through<ACT, V>(k, act, d, st, (uint64_t)(from + (int64_t)p * s.c + ch), h,
                    g);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -419,7 +421,7 @@ __global__ __launch_bounds__(BLOCK) void gn_bwd_sums(
     __syncthreads();
   }
   for (int g = threadIdx.x; g < s.g; g += BLOCK)
-    part_g[((int64_t)b * s.g + g) * splits + split] =
+    part_g[((int64_t)b * s.g + g) * cut.n + split] =
         make_float2(joined[g], joined[s.g + g]);
 }
 
@@ -461,28 +463,28 @@ __global__ __launch_bounds__(BLOCK) void gn_param_grad(
 
 // The first `param_blocks` blocks sum the parameters' gradients while the
 // others, (chunk, sample), write dx.
-template <typename T, int V>
+template <typename T, int V, int ACT>
 __global__ __launch_bounds__(BLOCK) void gn_bwd_dx(
     const T* __restrict__ x, const T* __restrict__ gy, T* __restrict__ dx,
     const float* __restrict__ w, const float* __restrict__ bias,
     const float* __restrict__ mean, const float* __restrict__ rstd,
     const float* __restrict__ part_c, const float2* __restrict__ part_g,
-    float* __restrict__ db, float* __restrict__ dw, Shape s, int splits,
-    int chunks, int param_blocks, int act, DropoutArgs d) {
+    float* __restrict__ db, float* __restrict__ dw, Shape s, Cut cut,
+    Cut chunks, int param_blocks, int act, DropoutArgs d) {
   extern __shared__ float sums[];  // [2][g], at least BLOCK
   if ((int)blockIdx.x < param_blocks) {
-    param_sums(part_c, (int64_t)s.b * splits, s.c, blockIdx.x, db, dw, sums);
+    param_sums(part_c, (int64_t)s.b * cut.n, s.c, blockIdx.x, db, dw, sums);
     return;
   }
   const int at_block = blockIdx.x - param_blocks;
-  const int chunk = at_block % chunks, b = at_block / chunks;
+  const int chunk = at_block % chunks.n, b = at_block / chunks.n;
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
   const DropoutState st = dropout_state(d);
   const float inv_n = 1.0f / ((float)s.hw * (float)s.cg);
   for (int g = wave; g < s.g; g += BLOCK / WAVE) {
-    const float2* e = part_g + ((int64_t)b * s.g + g) * splits;
+    const float2* e = part_g + ((int64_t)b * s.g + g) * cut.n;
     float t1 = 0.0f, t2 = 0.0f;
-    for (int i = lane; i < splits; i += WAVE) {
+    for (int i = lane; i < cut.n; i += WAVE) {
       t1 += e[i].x;
       t2 += e[i].y;
     }
@@ -496,9 +498,8 @@ __global__ __launch_bounds__(BLOCK) void gn_bwd_dx(
   __syncthreads();
   mean += (int64_t)b * s.g;
   rstd += (int64_t)b * s.g;
-  const int64_t p0 = split_at(s.hw, chunk, chunks);
-  const int pixels = (int)(split_at(s.hw, chunk + 1, chunks) - p0);
-  const int64_t from = ((int64_t)b * s.hw + p0) * s.c;
+  const int pixels = chunks.pixels(chunk);
+  const int64_t from = ((int64_t)b * s.hw + chunks.first(chunk)) * s.c;
   const int nv = s.c / V;
   for (int c0 = 0; c0 < nv; c0 += BLOCK) {
     const int cols = min(BLOCK, nv - c0);
@@ -519,7 +520,7 @@ __global__ __launch_bounds__(BLOCK) void gn_bwd_dx(
       unpack<T, V>(rx, h);
       unpack<T, V>(rg, g);
       const int64_t at = from + (int64_t)p * s.c + ch;
-      through<V>(k, act, d, st, (uint64_t)at, h, g);
+      through<ACT, V>(k, act, d, st, (uint64_t)at, h, g);
 #pragma unroll
       for (int j = 0; j < V; ++j)
         g[j] = k.rstd[j] * (fmaf(k.w[j], g[j], -t1[j]) - h[j] * t2[j]);
@@ -596,26 +597,43 @@ int vector_of(const Shape& s, std::initializer_list<const void*> ptrs) {
 
 // Blocks per sample: about `total` blocks over the batch, each with `least`
 // values or more, and at most `most` (each costs the second launch a read).
-int split_count(const Shape& s, int total, int64_t least, int most) {
+Cut cut_pixels(const Shape& s, int total, int64_t least, int most) {
   int64_t n = (total + s.b - 1) / s.b;
   n = std::min<int64_t>(n, std::max<int64_t>(1, s.hw * s.c / least));
   n = std::min<int64_t>(n, s.hw);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(n, most));
+  n = std::max<int64_t>(1, std::min<int64_t>(n, most));
+  return {(int)n, (int)(s.hw / n), (int)(s.hw % n)};
 }
 
-#define GN_VECTOR(V_, ...)                    \
-  do {                                        \
-    if (V_ == 8) {                            \
-      constexpr int V = 8;                    \
-      __VA_ARGS__;                            \
-    } else if (V_ == 4) {                     \
-      constexpr int V = 4;                    \
-      __VA_ARGS__;                            \
-    } else {                                  \
-      constexpr int V = 1;                    \
-      __VA_ARGS__;                            \
-    }                                         \
+// Activations are compiled in for whole vectors; narrower ones, which odd
+// channel counts take, choose as they go.
+#define GN_VARIANT(V_, ACT_, ...)                                    \
+  do {                                                               \
+    if (V_ == 8) {                                                   \
+      constexpr int V = 8;                                           \
+      switch (ACT_) {                                                \
+        case ACT_ELU: { constexpr int ACT = ACT_ELU; __VA_ARGS__; break; }     \
+        case ACT_LEAKY: { constexpr int ACT = ACT_LEAKY; __VA_ARGS__; break; } \
+        case ACT_RELU: { constexpr int ACT = ACT_RELU; __VA_ARGS__; break; }   \
+        case ACT_SILU: { constexpr int ACT = ACT_SILU; __VA_ARGS__; break; }   \
+        default: { constexpr int ACT = ACT_NONE; __VA_ARGS__; break; }         \
+      }                                                              \
+    } else if (V_ == 4) {                                            \
+      constexpr int V = 4, ACT = ACT_ANY;                            \
+      __VA_ARGS__;                                                   \
+    } else {                                                         \
+      constexpr int V = 1, ACT = ACT_ANY;                            \
+      __VA_ARGS__;                                                   \
+    }                                                                \
   } while (0)
+
+template <typename T, int V>
+void launch_stats(const T* x, float2* part, const Shape& s, const Cut& cut,
+                  hipStream_t stream) {
+  auto kernel = s.cg % V == 0 ? gn_stats<T, V, true> : gn_stats<T, V, false>;
+  kernel<<<s.b * cut.n, BLOCK, 3 * s.g * 4, stream>>>(x, part, s, cut);
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+}
 
 template <typename T>
 void forward(const at::Tensor& x, at::Tensor& y, const float* w,
@@ -625,23 +643,22 @@ void forward(const at::Tensor& x, at::Tensor& y, const float* w,
   const T* px = (const T*)x.data_ptr();
   T* py = (T*)y.data_ptr();
   const int v = vector_of<T>(s, {px, py});
-  const int splits = split_count(s, 2048, 16384, 256);
-  const int chunks = split_count(s, 2048, 16384, 1 << 20);
-  TORCH_CHECK((int64_t)s.b * std::max(splits, chunks) < (1ll << 31),
+  const Cut cut = cut_pixels(s, 2048, 16384, 256);
+  const Cut chunks = cut_pixels(s, 2048, 16384, 1 << 20);
+  TORCH_CHECK((int64_t)s.b * std::max(cut.n, chunks.n) < (1ll << 31),
               "group_norm: tensor too large");
-  auto part = at::empty({(int64_t)s.b * s.g * splits * 2}, mean.options());
+  auto part = at::empty({(int64_t)s.b * s.g * cut.n * 2}, mean.options());
   float2* pp = (float2*)part.data_ptr();
-  GN_VECTOR(v, {
-    if (s.cg % V == 0)
-      gn_stats<T, V, true><<<s.b * splits, BLOCK, 3 * s.g * 4, stream>>>(
-          px, pp, s, splits);
-    else
-      gn_stats<T, V, false><<<s.b * splits, BLOCK, 3 * s.g * 4, stream>>>(
-          px, pp, s, splits);
-    C10_HIP_KERNEL_LAUNCH_CHECK();
-    gn_apply<T, V><<<s.b * chunks, BLOCK, 2 * s.g * 4, stream>>>(
+  if (v == 8)
+    launch_stats<T, 8>(px, pp, s, cut, stream);
+  else if (v == 4)
+    launch_stats<T, 4>(px, pp, s, cut, stream);
+  else
+    launch_stats<T, 1>(px, pp, s, cut, stream);
+  GN_VARIANT(v, act, {
+    gn_apply<T, V, ACT><<<s.b * chunks.n, BLOCK, 2 * s.g * 4, stream>>>(
         px, py, w, bias, pp, mean.data_ptr<float>(), rstd.data_ptr<float>(), s,
-        splits, chunks, eps, act, d);
+        cut, chunks, eps, act, d);
     C10_HIP_KERNEL_LAUNCH_CHECK();
   });
 }
@@ -655,29 +672,29 @@ void backward(const at::Tensor& x, const at::Tensor& gy, T* dx, const float* w,
   const T* px = (const T*)x.data_ptr();
   const T* pg = (const T*)gy.data_ptr();
   const int v = vector_of<T>(s, {px, pg, dx});
-  const int splits = split_count(s, 2048, 16384, 256);
-  const int chunks = split_count(s, 2048, 16384, 1 << 20);
+  const Cut cut = cut_pixels(s, 2048, 16384, 256);
+  const Cut chunks = cut_pixels(s, 2048, 16384, 1 << 20);
   const int param_blocks = db || dw ? (s.c + 7) / 8 : 0;
-  TORCH_CHECK((int64_t)s.b * std::max(splits, chunks) + param_blocks <
+  TORCH_CHECK((int64_t)s.b * std::max(cut.n, chunks.n) + param_blocks <
                   (1ll << 31),
               "group_norm: tensor too large");
   const auto opts = x.options().dtype(at::kFloat);
-  auto part_c = at::empty({2 * (int64_t)s.b * splits * s.c}, opts);
-  auto part_g = at::empty({(int64_t)s.b * s.g * splits * 2}, opts);
+  auto part_c = at::empty({2 * (int64_t)s.b * cut.n * s.c}, opts);
+  auto part_g = at::empty({(int64_t)s.b * s.g * cut.n * 2}, opts);
   float* pc = part_c.data_ptr<float>();
   float2* pp = (float2*)part_g.data_ptr();
-  GN_VECTOR(v, {
-    gn_bwd_sums<T, V><<<s.b * splits, BLOCK, 2 * s.g * 4, stream>>>(
-        px, pg, w, bias, mean, rstd, pc, pp, s, splits, act, d);
+  GN_VARIANT(v, act, {
+    gn_bwd_sums<T, V, ACT><<<s.b * cut.n, BLOCK, 2 * s.g * 4, stream>>>(
+        px, pg, w, bias, mean, rstd, pc, pp, s, cut, act, d);
     C10_HIP_KERNEL_LAUNCH_CHECK();
     if (dx) {
-      gn_bwd_dx<T, V><<<s.b * chunks + param_blocks, BLOCK,
-                        std::max(2 * s.g, BLOCK) * 4, stream>>>(
-          px, pg, dx, w, bias, mean, rstd, pc, pp, db, dw, s, splits, chunks,
+      gn_bwd_dx<T, V, ACT><<<s.b * chunks.n + param_blocks, BLOCK,
+                             std::max(2 * s.g, BLOCK) * 4, stream>>>(
+          px, pg, dx, w, bias, mean, rstd, pc, pp, db, dw, s, cut, chunks,
           param_blocks, act, d);
     } else {
       gn_param_grad<<<param_blocks, BLOCK, 0, stream>>>(
-          pc, (int64_t)s.b * splits, s.c, db, dw);
+          pc, (int64_t)s.b * cut.n, s.c, db, dw);
     }
     C10_HIP_KERNEL_LAUNCH_CHECK();
   });

@@ -41,14 +41,18 @@ __device__ __forceinline__ DropoutState dropout_state(const DropoutArgs& d) {
           (uint32_t)(offset >> 32)};
 }
 
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);  // one instruction
+}
+
 __device__ __forceinline__ void philox4x32(uint32_t c[4], uint32_t k0,
                                            uint32_t k1) {
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t a = (uint64_t)c[0] * 0xD2511F53u;
     const uint64_t b = (uint64_t)c[2] * 0xCD9E8D57u;
-    const uint32_t n0 = (uint32_t)(b >> 32) ^ c[1] ^ k0;
-    const uint32_t n2 = (uint32_t)(a >> 32) ^ c[3] ^ k1;
+    const uint32_t n0 = xor3((uint32_t)(b >> 32), c[1], k0);
+    const uint32_t n2 = xor3((uint32_t)(a >> 32), c[3], k1);
     c[0] = n0;
     c[1] = (uint32_t)b;
     c[2] = n2;

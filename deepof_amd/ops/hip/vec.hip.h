@@ -22,8 +22,20 @@ __device__ __forceinline__ void unpack(const Pack<T, V>& p, float (&f)[V]) {
 template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> pack(const float (&f)[V]) {
   Pack<T, V> p;
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    // two at a time: one instruction converts a pair to bf16
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef T t16x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-  for (int k = 0; k < V; ++k) p.v[k] = (T)f[k];
+    for (int k = 0; k < V; k += 2) {
+      const f32x2 pair = {f[k], f[k + 1]};
+      *reinterpret_cast<t16x2*>(&p.v[k]) =
+          __builtin_convertvector(pair, t16x2);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) p.v[k] = (T)f[k];
+  }
   return p;
 }
 
@@ -37,7 +49,9 @@ __device__ __forceinline__ void store_pack(T* at, const Pack<T, V>& p) {
   *reinterpret_cast<Pack<T, V>*>(at) = p;
 }
 
-enum Act { ACT_NONE = 0, ACT_ELU = 1, ACT_LEAKY = 2, ACT_RELU = 3, ACT_SILU = 4 };
+// ACT_ANY: not known at compile time, passed in.
+enum Act { ACT_ANY = -1, ACT_NONE = 0, ACT_ELU = 1, ACT_LEAKY = 2, ACT_RELU = 3,
+           ACT_SILU = 4 };
 
 // e^z through the hardware's 2^t.  t = z log2(e) is carried in two floats,
 // or its rounding would cost |z| 2^-24 of the result.
@@ -74,9 +88,9 @@ __device__ __forceinline__ float expm1_neg(float z) {
 }
 
 // v = act(v).  Comparisons are written so that NaN stays NaN.
-template <typename T, int V>
+template <typename T, int ACT, int V>
 __device__ __forceinline__ void act_apply(int act, float (&v)[V]) {
-  switch (act) {
+  switch (ACT == ACT_ANY ? act : ACT) {
     case ACT_ELU:
 #pragma unroll
       for (int k = 0; k < V; ++k) v[k] = v[k] <= 0.0f ? expm1_neg<T>(v[k]) : v[k];
@@ -100,10 +114,10 @@ __device__ __forceinline__ void act_apply(int act, float (&v)[V]) {
 }
 
 // g *= act'(z)
-template <int V>
+template <int ACT, int V>
 __device__ __forceinline__ void act_backward(int act, const float (&z)[V],
                                              float (&g)[V]) {
-  switch (act) {
+  switch (ACT == ACT_ANY ? act : ACT) {
     case ACT_ELU:
 #pragma unroll
       for (int k = 0; k < V; ++k) g[k] = z[k] <= 0.0f ? g[k] * exp_f32(z[k]) : g[k];
