@@ -299,23 +299,6 @@ def _dense_format(x):
     return torch.contiguous_format
 
 
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, p, rng, seed, offset, act):
-        ctx.save_for_backward(x if act else None, rng)
-        ctx.meta = (p, seed, offset, act, _dense_format(x))
-        return require_hip().dropout_forward(x, act, p, rng, seed, offset)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gy):
-        x, rng = ctx.saved_tensors
-        p, seed, offset, act, fmt = ctx.meta
-        gx = require_hip().dropout_backward(
-            gy.contiguous(memory_format=fmt), x, act, p, rng, seed, offset)
-        return gx, None, None, None, None, None
-
-
 def dropout(x: torch.Tensor, p: float = 0.5, rng=None,
             act: str | None = None) -> torch.Tensor:
     """act(x) / (1 - p) where kept, 0 where dropped (with probability p).
@@ -335,30 +318,7 @@ def dropout(x: torch.Tensor, p: float = 0.5, rng=None,
     x = x.contiguous(memory_format=_dense_format(x))
     if not x.is_cuda:
         return ref.dropout(x, p, _rng_tensor(rng, seed, offset), act)
-    code = _ACT_CODES[act]
-    if x.requires_grad and torch.is_grad_enabled():
-        return _Dropout.apply(x, p, rng, seed, offset, code)
-    return require_hip().dropout_forward(x, code, p, rng, seed, offset)
-
-
-class _GroupNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, act, p, rng, seed, offset):
-        y, mean, rstd = require_hip().group_norm_forward(
-            x, groups, weight, bias, eps, act, p, rng, seed, offset)
-        ctx.save_for_backward(x, weight, bias, mean, rstd, rng)
-        ctx.meta = (act, p, seed, offset)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gy):
-        x, weight, bias, mean, rstd, rng = ctx.saved_tensors
-        act, p, seed, offset = ctx.meta
-        gx, gw, gb = require_hip().group_norm_backward(
-            gy.contiguous(memory_format=torch.channels_last), x, weight, bias,
-            mean, rstd, act, p, rng, seed, offset, *ctx.needs_input_grad[:3])
-        return (gx, gw, gb) + (None,) * 7
+    return require_hip().dropout(x, _ACT_CODES[act], p, rng, seed, offset)
 
 
 def group_norm(x: torch.Tensor, num_groups: int,
@@ -403,10 +363,5 @@ def group_norm(x: torch.Tensor, num_groups: int,
     # the kernels read fp32 parameters; a cast is part of the graph
     weight = None if weight is None else weight.float().contiguous()
     bias = None if bias is None else bias.float().contiguous()
-    code = _ACT_CODES[act]
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, bias)):
-        return _GroupNorm.apply(x, weight, bias, num_groups, eps, code, p, rng,
-                                seed, offset)
-    return require_hip().group_norm_forward(
-        x, num_groups, weight, bias, eps, code, p, rng, seed, offset)[0]
+    return require_hip().group_norm(x, num_groups, weight, bias, eps,
+                                    _ACT_CODES[act], p, rng, seed, offset)

@@ -1,0 +1,147 @@
+// Group norm and dropout as differentiable calls.  The nodes are C++: a
+// Python function's backward would take the interpreter's lock from the
+// engine's thread, some 20 us that small activations feel.
+
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/extension.h>
+
+using at::Tensor;
+using OptTensor = c10::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+std::vector<Tensor> group_norm_forward(const Tensor& x, int64_t groups,
+                                       const Tensor& weight,
+                                       const Tensor& bias, double eps,
+                                       int64_t act, double p,
+                                       const Tensor& rng, int64_t seed,
+                                       int64_t offset, bool keep_stats);
+std::vector<Tensor> group_norm_backward(const Tensor& gy, const Tensor& x,
+                                        const Tensor& weight,
+                                        const Tensor& bias,
+                                        const Tensor& stats, int64_t act,
+                                        double p, const Tensor& rng,
+                                        int64_t seed, int64_t offset,
+                                        bool need_x, bool need_weight,
+                                        bool need_bias);
+Tensor dropout_forward(const Tensor& x, int64_t act, double p,
+                       const Tensor& rng, int64_t seed, int64_t offset);
+Tensor dropout_backward(const Tensor& gy, const Tensor& x, int64_t act,
+                        double p, const Tensor& rng, int64_t seed,
+                        int64_t offset);
+
+namespace {
+
+// Gradients of gradients are not provided: where a graph of the gradients is
+// being built, they carry a node that says so when it is reached.
+variable_list once(variable_list grads, std::initializer_list<Tensor> from) {
+  if (!at::GradMode::is_enabled()) return grads;
+  bool any = false;
+  for (const Tensor& t : from) any = any || (t.defined() && t.requires_grad());
+  if (!any) return grads;
+  for (Tensor& g : grads)
+    if (g.defined()) g = g.detach().requires_grad_(true);
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      "deepof_amd: this gradient cannot be differentiated again",
+      (int64_t)grads.size());
+  return (*error)(std::move(grads));
+}
+
+struct GroupNorm : torch::autograd::Function<GroupNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x,
+                        const OptTensor& weight, const OptTensor& bias,
+                        int64_t groups, double eps, int64_t act, double p,
+                        const OptTensor& rng, int64_t seed, int64_t offset) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor r = rng.value_or(Tensor());
+    const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+    auto out = group_norm_forward(x, groups, w, b, eps, act, p, r, seed, offset,
+                                  true);
+    ctx->save_for_backward({x, w, b, out[1], r});
+    ctx->saved_data["a"] = act;
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["s"] = seed;
+    ctx->saved_data["o"] = offset;
+    return out[0];
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list gy) {
+    const auto s = ctx->get_saved_variables();
+    variable_list g;
+    // edges are those of the tensors that were there
+    const bool has_w = s[1].defined(), has_b = s[2].defined();
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      g = group_norm_backward(
+          gy[0].contiguous(at::MemoryFormat::ChannelsLast), s[0], s[1], s[2],
+          s[3], ctx->saved_data["a"].toInt(), ctx->saved_data["p"].toDouble(),
+          s[4], ctx->saved_data["s"].toInt(), ctx->saved_data["o"].toInt(),
+          ctx->needs_input_grad(0), has_w && ctx->needs_input_grad(1),
+          has_b && ctx->needs_input_grad(has_w ? 2 : 1));
+    }
+    g = once(std::move(g), {gy[0], s[0], s[1], s[2]});
+    g.resize(10);
+    return g;
+  }
+};
+
+at::MemoryFormat dense_format(const Tensor& x) {
+  return !x.is_contiguous() && x.is_contiguous(at::MemoryFormat::ChannelsLast)
+             ? at::MemoryFormat::ChannelsLast
+             : at::MemoryFormat::Contiguous;
+}
+
+struct Dropout : torch::autograd::Function<Dropout> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, int64_t act,
+                        double p, const OptTensor& rng, int64_t seed,
+                        int64_t offset) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor r = rng.value_or(Tensor());
+    ctx->save_for_backward({act ? x : Tensor(), r});
+    ctx->saved_data["a"] = act;
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["s"] = seed;
+    ctx->saved_data["o"] = offset;
+    ctx->saved_data["f"] = (int64_t)dense_format(x);
+    return dropout_forward(x, act, p, r, seed, offset);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list gy) {
+    const auto s = ctx->get_saved_variables();
+    const auto format = (at::MemoryFormat)ctx->saved_data["f"].toInt();
+    Tensor g;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      g = dropout_backward(gy[0].contiguous(format), s[0],
+                           ctx->saved_data["a"].toInt(),
+                           ctx->saved_data["p"].toDouble(), s[1],
+                           ctx->saved_data["s"].toInt(),
+                           ctx->saved_data["o"].toInt());
+    }
+    variable_list out = once({g}, {gy[0], s[0]});
+    out.resize(6);
+    return out;
+  }
+};
+
+bool wanted(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+}  // namespace
+
+Tensor group_norm(const Tensor& x, int64_t groups, const OptTensor& weight,
+                  const OptTensor& bias, double eps, int64_t act, double p,
+                  const OptTensor& rng, int64_t seed, int64_t offset) {
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  if (at::GradMode::is_enabled() && (wanted(x) || wanted(w) || wanted(b)))
+    return GroupNorm::apply(x, weight, bias, groups, eps, act, p, rng, seed,
+                            offset);
+  return group_norm_forward(x, groups, w, b, eps, act, p,
+                            rng.value_or(Tensor()), seed, offset, false)[0];
+}
+
+Tensor dropout(const Tensor& x, int64_t act, double p, const OptTensor& rng,
+               int64_t seed, int64_t offset) {
+  if (at::GradMode::is_enabled() && wanted(x))
+    return Dropout::apply(x, act, p, rng, seed, offset);
+  return dropout_forward(x, act, p, rng.value_or(Tensor()), seed, offset);
+}

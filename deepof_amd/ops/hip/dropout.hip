@@ -21,8 +21,9 @@ constexpr int BLOCK = 256;
 constexpr int UNROLL = 2;  // vectors of 8 in flight per thread
 
 template <typename T, bool WIDE>
-__device__ __forceinline__ Pack<T, 8> load8(const T* at, int count) {
-  if (WIDE && count == 8) return load_pack<T, 8>(at);
+__device__ __forceinline__ Pack<T, 8> load8(const T* at, int count,
+                                            bool stream) {
+  if (WIDE && count == 8) return load_pack<T, 8>(at, stream);
   Pack<T, 8> p;
 #pragma unroll
   for (int k = 0; k < 8; ++k) p.v[k] = k < count ? at[k] : (T)0.0f;
@@ -34,7 +35,7 @@ __device__ __forceinline__ Pack<T, 8> load8(const T* at, int count) {
 template <typename T, bool WIDE, bool BACK, int ACT>
 __global__ __launch_bounds__(BLOCK) void dropout_kernel(
     const T* __restrict__ x, const T* __restrict__ gy, T* __restrict__ out,
-    int64_t n, int act, DropoutArgs d) {
+    int64_t n, int act, bool stream, DropoutArgs d) {
   const bool need_x = !BACK || (ACT == ACT_ANY ? act : ACT) != ACT_NONE;
   const DropoutState st = dropout_state(d);
   const int64_t first = (int64_t)blockIdx.x * (BLOCK * UNROLL) + threadIdx.x;
@@ -44,8 +45,8 @@ __global__ __launch_bounds__(BLOCK) void dropout_kernel(
     const int64_t at = (first + i * BLOCK) * 8;
     const int count = (int)min((int64_t)8, n - at);
     if (count <= 0) continue;
-    if (need_x) rx[i] = load8<T, WIDE>(x + at, count);
-    if (BACK) rg[i] = load8<T, WIDE>(gy + at, count);
+    if (need_x) rx[i] = load8<T, WIDE>(x + at, count, stream);
+    if (BACK) rg[i] = load8<T, WIDE>(gy + at, count, stream);
   }
 #pragma unroll
   for (int i = 0; i < UNROLL; ++i) {
@@ -67,7 +68,7 @@ __global__ __launch_bounds__(BLOCK) void dropout_kernel(
     if (d.on) dropout_apply<8>(d, st, (uint64_t)at, v);
     const Pack<T, 8> o = pack<T, 8>(v);
     if (WIDE && count == 8) {
-      store_pack<T, 8>(out + at, o);
+      store_pack<T, 8>(out + at, o, stream);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
@@ -95,8 +96,9 @@ void launch(const void* x, const void* gy, void* out, int64_t n, int act,
       default: kernel = dropout_kernel<T, true, BACK, ACT_NONE>; break;
     }
   }
-  kernel<<<(unsigned)blocks, BLOCK, 0, stream>>>(
-      (const T*)x, (const T*)gy, (T*)out, n, act, d);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(BLOCK), 0, stream,
+                     (const T*)x, (const T*)gy, (T*)out, n, act, n *
+                     (int64_t)sizeof(T) > STREAM_BYTES, d);
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
@@ -139,8 +141,8 @@ void check_dense(const at::Tensor& t, const char* name) {
 
 }  // namespace
 
-at::Tensor dropout_forward(at::Tensor x, long act, double p,
-                           c10::optional<at::Tensor> rng, int64_t seed,
+at::Tensor dropout_forward(const at::Tensor& x, int64_t act, double p,
+                           const at::Tensor& rng, int64_t seed,
                            int64_t offset) {
   check_dense(x, "x");
   c10::DeviceGuard guard(x.device());
@@ -148,21 +150,22 @@ at::Tensor dropout_forward(at::Tensor x, long act, double p,
                      dropout_args(p, rng, seed, offset, x));
 }
 
-at::Tensor dropout_backward(at::Tensor gy, c10::optional<at::Tensor> x,
-                            long act, double p, c10::optional<at::Tensor> rng,
+// x is read where the activation has a slope, and may be undefined elsewhere.
+at::Tensor dropout_backward(const at::Tensor& gy, const at::Tensor& x,
+                            int64_t act, double p, const at::Tensor& rng,
                             int64_t seed, int64_t offset) {
   check_dense(gy, "gy");
   c10::DeviceGuard guard(gy.device());
   const void* xp = nullptr;
   if (act != ACT_NONE) {
     const auto cl = at::MemoryFormat::ChannelsLast;
-    TORCH_CHECK(x.has_value() && x->sizes() == gy.sizes() &&
-                    ((x->is_contiguous() && gy.is_contiguous()) ||
-                     (x->is_contiguous(cl) && gy.is_contiguous(cl))) &&
-                    x->scalar_type() == gy.scalar_type() &&
-                    x->device() == gy.device(),
+    TORCH_CHECK(x.defined() && x.sizes() == gy.sizes() &&
+                    ((x.is_contiguous() && gy.is_contiguous()) ||
+                     (x.is_contiguous(cl) && gy.is_contiguous(cl))) &&
+                    x.scalar_type() == gy.scalar_type() &&
+                    x.device() == gy.device(),
                 "dropout: x must be like gy");
-    xp = x->data_ptr();
+    xp = x.data_ptr();
   }
   return dropout_any(gy, xp, gy.data_ptr(), act,
                      dropout_args(p, rng, seed, offset, gy));

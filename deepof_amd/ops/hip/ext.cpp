@@ -45,21 +45,15 @@ void fused_adam(std::vector<at::Tensor> params, std::vector<at::Tensor> grads,
                 std::vector<at::Tensor> exp_avg_sqs, double lr, double beta1,
                 double beta2, double eps, double wd, double bias1,
                 double bias2);
-std::vector<at::Tensor> group_norm_forward(
-    at::Tensor x, int64_t groups, c10::optional<at::Tensor> weight,
-    c10::optional<at::Tensor> bias, double eps, int64_t act, double p,
-    c10::optional<at::Tensor> rng, int64_t seed, int64_t offset);
-std::vector<at::Tensor> group_norm_backward(
-    at::Tensor gy, at::Tensor x, c10::optional<at::Tensor> weight,
-    c10::optional<at::Tensor> bias, at::Tensor mean, at::Tensor rstd,
-    int64_t act, double p, c10::optional<at::Tensor> rng, int64_t seed,
-    int64_t offset, bool need_x, bool need_weight, bool need_bias);
-at::Tensor dropout_forward(at::Tensor x, long act, double p,
-                           c10::optional<at::Tensor> rng, int64_t seed,
-                           int64_t offset);
-at::Tensor dropout_backward(at::Tensor gy, c10::optional<at::Tensor> x,
-                            long act, double p, c10::optional<at::Tensor> rng,
-                            int64_t seed, int64_t offset);
+at::Tensor group_norm(const at::Tensor& x, int64_t groups,
+                      const c10::optional<at::Tensor>& weight,
+                      const c10::optional<at::Tensor>& bias, double eps,
+                      int64_t act, double p,
+                      const c10::optional<at::Tensor>& rng, int64_t seed,
+                      int64_t offset);
+at::Tensor dropout(const at::Tensor& x, int64_t act, double p,
+                   const c10::optional<at::Tensor>& rng, int64_t seed,
+                   int64_t offset);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("warp_forward", &warp_forward, "bilinear backward warp (fwd)");
@@ -90,12 +84,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "gather all 4 parity sub-filters of a transposed conv");
   m.def("conv2d_fwd_subpixel4", &conv2d_fwd_subpixel4,
         "all-parity sub-pixel transposed conv in one launch");
-  m.def("group_norm_forward", &group_norm_forward,
-        "group norm + act (+ dropout), channels last -> y, mean, rstd");
-  m.def("group_norm_backward", &group_norm_backward,
-        "group norm backward -> dx, dweight, dbias");
-  m.def("dropout_forward", &dropout_forward,
-        "act + dropout, mask from a counter-based generator");
-  m.def("dropout_backward", &dropout_backward,
-        "gradient of act + dropout, the mask computed again");
+  m.def("group_norm", &group_norm,
+        "group norm + act (+ dropout), channels last, differentiable");
+  m.def("dropout", &dropout,
+        "act + dropout, mask from a counter-based generator, differentiable");
 }

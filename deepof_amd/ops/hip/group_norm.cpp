@@ -1,0 +1,111 @@
+// Group norm: checks, allocations and the choice of type.  The mathematics and
+// the kernels are in group_norm.hip.h.
+
+#include "group_norm.h"
+
+#include <c10/core/DeviceGuard.h>
+
+namespace {
+
+constexpr int MAX_GROUPS = 4096;  // their sums live in LDS
+
+GroupNormShape shape_of(const at::Tensor& x, int64_t groups) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 4 &&
+                  x.is_contiguous(at::MemoryFormat::ChannelsLast),
+              "group_norm: x must be a 4-D channels-last GPU tensor");
+  TORCH_CHECK(groups >= 1 && groups <= MAX_GROUPS && x.size(1) >= 1 &&
+                  x.size(1) % groups == 0,
+              "group_norm: the channels must divide into 1 to ", MAX_GROUPS,
+              " groups");
+  TORCH_CHECK(x.size(0) < (1ll << 24) && x.size(1) < (1ll << 24) &&
+                  x.size(2) * x.size(3) < (1ll << 30),
+              "group_norm: tensor too large");
+  GroupNormShape s;
+  s.hw = x.size(2) * x.size(3);
+  s.b = (int)x.size(0);
+  s.c = (int)x.size(1);
+  s.g = (int)groups;
+  s.cg = s.c / s.g;
+  return s;
+}
+
+const float* param(const at::Tensor& t, const at::Tensor& x,
+                   const char* name) {
+  if (!t.defined()) return nullptr;
+  TORCH_CHECK(t.scalar_type() == at::kFloat && t.is_contiguous() &&
+                  t.dim() == 1 && t.size(0) == x.size(1) &&
+                  t.device() == x.device(),
+              "group_norm: ", name, " must be C floats on the input's device");
+  return t.data_ptr<float>();
+}
+
+#define GN_TYPE(t, call, args)                                              \
+  switch (t) {                                                              \
+    case at::kFloat: call##f32 args; break;                                 \
+    case at::kHalf: call##f16 args; break;                                  \
+    case at::kBFloat16: call##bf16 args; break;                             \
+    default:                                                                \
+      TORCH_CHECK(false,                                                    \
+                  "group_norm: float32, float16 or bfloat16 expected");     \
+  }
+
+}  // namespace
+
+// -> y, and stats (mean and rstd, [2, B, G]) where asked for
+std::vector<at::Tensor> group_norm_forward(
+    const at::Tensor& x, int64_t groups, const at::Tensor& weight,
+    const at::Tensor& bias, double eps, int64_t act, double p,
+    const at::Tensor& rng, int64_t seed, int64_t offset, bool keep_stats) {
+  const GroupNormShape s = shape_of(x, groups);
+  TORCH_CHECK(eps > 0.0, "group_norm: eps must be positive");
+  c10::DeviceGuard guard(x.device());
+  const DropoutArgs d = dropout_args(p, rng, seed, offset, x);
+  const float* w = param(weight, x, "weight");
+  const float* b = param(bias, x, "bias");
+  auto y = at::empty_like(x, x.options(), at::MemoryFormat::ChannelsLast);
+  at::Tensor stats;
+  if (keep_stats)
+    stats = at::empty({2, x.size(0), groups}, x.options().dtype(at::kFloat));
+  float* kept = keep_stats ? stats.data_ptr<float>() : nullptr;
+  if (x.numel() > 0)
+    GN_TYPE(x.scalar_type(),
+            gn_forward_, (x, y, w, b, kept, s, (float)eps, (int)act, d));
+  return {y, stats};
+}
+
+// -> dx, dweight, dbias; an undefined tensor where none is wanted
+std::vector<at::Tensor> group_norm_backward(
+    const at::Tensor& gy, const at::Tensor& x, const at::Tensor& weight,
+    const at::Tensor& bias, const at::Tensor& stats, int64_t act, double p,
+    const at::Tensor& rng, int64_t seed, int64_t offset, bool need_x,
+    bool need_weight, bool need_bias) {
+  TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() &&
+                  stats.dim() == 3 && stats.size(0) == 2 &&
+                  stats.size(1) == x.size(0) && stats.device() == x.device(),
+              "group_norm: stats must be [2, B, G] floats");
+  const GroupNormShape s = shape_of(x, stats.size(2));
+  TORCH_CHECK(gy.sizes() == x.sizes() && gy.scalar_type() == x.scalar_type() &&
+                  gy.device() == x.device() &&
+                  gy.is_contiguous(at::MemoryFormat::ChannelsLast),
+              "group_norm: gy must be like x");
+  c10::DeviceGuard guard(x.device());
+  const DropoutArgs d = dropout_args(p, rng, seed, offset, x);
+  const float* w = param(weight, x, "weight");
+  const float* b = param(bias, x, "bias");
+  at::Tensor dx, dw, db;
+  const auto opts = x.options().dtype(at::kFloat);
+  if (need_x) dx = at::empty_like(x, x.options(), at::MemoryFormat::ChannelsLast);
+  if (need_weight) dw = at::empty({x.size(1)}, opts);
+  if (need_bias) db = at::empty({x.size(1)}, opts);
+  if (x.numel() == 0) {
+    if (need_weight) dw.zero_();
+    if (need_bias) db.zero_();
+    return {dx, dw, db};
+  }
+  if (!need_x && !need_weight && !need_bias) return {dx, dw, db};
+  GN_TYPE(x.scalar_type(), gn_backward_,
+          (x, gy, dx, w, b, stats.data_ptr<float>(),
+           need_bias ? db.data_ptr<float>() : nullptr,
+           need_weight ? dw.data_ptr<float>() : nullptr, s, (int)act, d));
+  return {dx, dw, db};
+}

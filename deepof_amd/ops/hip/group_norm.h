@@ -1,0 +1,27 @@
+// Group norm's launches, per type of values.
+#pragma once
+
+#include <torch/extension.h>
+
+#include "dropout_args.h"
+
+struct GroupNormShape {
+  int64_t hw;
+  int b, c, g, cg;  // cg = c / g
+};
+
+// stat: [2][b][g], mean and rstd; written going forwards unless null.
+// dx, dw, db: null where not wanted.
+#define GN_DECLARE(NAME)                                                      \
+  void gn_forward_##NAME(const at::Tensor& x, at::Tensor& y, const float* w,  \
+                         const float* bias, float* stat,                      \
+                         const GroupNormShape& s, float eps, int act,         \
+                         const DropoutArgs& d);                               \
+  void gn_backward_##NAME(const at::Tensor& x, const at::Tensor& gy,          \
+                          at::Tensor& dx, const float* w, const float* bias,  \
+                          const float* stat, float* db, float* dw,            \
+                          const GroupNormShape& s, int act,                   \
+                          const DropoutArgs& d);
+GN_DECLARE(f32)
+GN_DECLARE(f16)
+GN_DECLARE(bf16)

@@ -1,0 +1,1211 @@
+// Group normalisation + affine + activation (+ dropout), channels last, for
+// gfx950: the kernels and their launches, for one type of values per file that
+// includes this.
+//
+// A group is the N = H W (C / G) values of one sample's C / G neighbouring
+// channels.  With mean and var of the group, rstd = 1 / sqrt(var + eps),
+// xhat = (x - mean) rstd and z = xhat w_c + b_c:
+//
+//   y    = act(z), with dropout behind it where asked for
+//   gz   = gy (through dropout) act'(z)
+//   db_c = sum gz,   dw_c = sum gz xhat       (over samples and pixels)
+//   s1   = sum w gz, s2   = sum w gz xhat     (over the group)
+//   dx   = rstd (w gz - (s1 + xhat s2) / N)
+//
+// z is computed again from x going backwards; mean and rstd, 2 B G floats,
+// are all that is kept.  Everything between loading x and storing y or dx is
+// fp32, and a result is rounded once.
+//
+// Memory bounds all of it.  Two routes:
+//  - tile: where a bundle of whole groups of a sample fits into half a CU's
+//    LDS, a block keeps it there, so that x (and gy) are read once, in one
+//    launch;
+//  - split: else pixels are split over blocks, which leave partial sums; a
+//    small launch joins them, and the last one reads x (and gy) again.
+// Keeping larger samples on the chip, a team of blocks each with its tile, was
+// built and measured too: a team's meeting costs its blocks some 20 us, in
+// which a CU's LDS holds far less than memory moves, and 64x64x192x256 bf16
+// took 390 us forwards against 290.
+//
+// Sums have a fixed order everywhere: no atomics, equal results every time.
+
+#pragma once
+
+#include <c10/hip/HIPException.h>
+#include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+#include <numeric>
+
+#include "group_norm.h"
+#include "philox.hip.h"
+#include "vec.hip.h"
+
+namespace {
+
+constexpr int WAVE = 64;
+constexpr int THREADS = 512;      // of a block that sums
+constexpr int BLOCK = 256;        // of a block that does not
+using Shape = GroupNormShape;
+
+// Pixels cut into n pieces, the first `more` of them one longer than `size`.
+struct Cut {
+  int n, size, more;
+  __device__ __forceinline__ int first(int i) const {
+    return i * size + min(i, more);
+  }
+  __device__ __forceinline__ int pixels(int i) const {
+    return size + (i < more ? 1 : 0);
+  }
+};
+
+// v + v of another lane: DPP moves within 16 lanes and between them, without
+// the journey through LDS that a shuffle takes.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(
+                 0, __float_as_int(v), CTRL, ROWS, 0xf, true));
+}
+
+// The sum over a wave, in every lane.
+__device__ __forceinline__ float wave_sum(float v) {
+  v = dpp_add<0xb1, 0xf>(v);   // lanes 1, 0, 3, 2
+  v = dpp_add<0x4e, 0xf>(v);   // lanes 2, 3, 0, 1
+  v = dpp_add<0x141, 0xf>(v);  // 8 lanes mirrored
+  v = dpp_add<0x140, 0xf>(v);  // 16 lanes mirrored
+  // the last lane of row 0 to row 1, of 2 to 3; then of rows 0, 1 to 2, 3
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x142,
+                                                  0xa, 0xf, false));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x143,
+                                                  0xc, 0xf, false));
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// f(j, group of channel ch + j) for j < V, with one division.
+template <int V, typename F>
+__device__ __forceinline__ void each_group(int ch, int cg, F f) {
+  int g = ch / cg, r = ch - g * cg;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    f(j, g);
+    if (++r == cg) {
+      r = 0;
+      ++g;
+    }
+  }
+}
+
+__device__ __forceinline__ float rstd_of(float m2, float n, float eps) {
+  return 1.0f / sqrtf(m2 / n + eps);
+}
+
+// Which part of some pixels by `cols` columns of V channels a thread works
+// on: one column, pixels row, row + rows, ...
+struct Place {
+  int cols, rows, row, col;
+  bool on;
+  __device__ __forceinline__ Place(int cols_, int threads) : cols(cols_) {
+    rows = threads / cols;
+    row = threadIdx.x / cols;
+    col = threadIdx.x - row * cols;
+    on = row < rows;
+  }
+  // pixels of this row among `pixels`
+  __device__ __forceinline__ int count(int pixels) const {
+    return on && row < pixels ? (pixels - row + rows - 1) / rows : 0;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// sums over a block
+// ---------------------------------------------------------------------------
+// A thread's V sums, one per channel, are first added up within the groups
+// that its vector touches: `units` of them, V / units channels each.  red
+// holds [thread][units] of F, float or float2.
+__device__ __forceinline__ void add_to(float& a, float b) { a += b; }
+__device__ __forceinline__ void add_to(float2& a, float2 b) {
+  a.x += b.x;
+  a.y += b.y;
+}
+__device__ __forceinline__ float over_wave(float v) { return wave_sum(v); }
+__device__ __forceinline__ float2 over_wave(float2 v) {
+  return make_float2(wave_sum(v.x), wave_sum(v.y));
+}
+
+template <int V, typename F>
+__device__ __forceinline__ void put_units(F* red, int units, const F (&s)[V]) {
+  F* at = red + threadIdx.x * units;
+  if (units == V) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) at[j] = s[j];
+  } else if (units == 1) {
+    F t = s[0];
+#pragma unroll
+    for (int j = 1; j < V; ++j) add_to(t, s[j]);
+    at[0] = t;
+  } else if (units == 2) {
+    F t0 = s[0], t1 = s[V / 2];
+#pragma unroll
+    for (int j = 1; j < V / 2; ++j) {
+      add_to(t0, s[j]);
+      add_to(t1, s[V / 2 + j]);
+    }
+    at[0] = t0;
+    at[1] = t1;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      F t = s[j];
+      add_to(t, s[j + (V > 1)]);
+      at[j / 2] = t;
+    }
+  }
+}
+
+// Sums red over the rows and over each group's units.  A row is `width` =
+// cols * units entries, of which unit `first` is the first in a group of `upg`
+// units; groups g0 .. lie in the row, possibly cut off at its ends.
+// done(group, sum) is called by one lane.
+template <typename F, typename Done>
+__device__ __forceinline__ void sum_groups(const F* red, const Place& pl,
+                                           int width, int first, int upg,
+                                           Done done) {
+  const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
+  const int last = first + width;
+  for (int g = first / upg + wave; g * upg < last; g += THREADS / WAVE) {
+    const int lo = max(g * upg, first) - first;
+    const int here = min((g + 1) * upg, last) - first - lo;
+    // a lane's next entry is 64 further: so many rows and so many units
+    const int skip_r = WAVE / here, skip_u = WAVE - skip_r * here;
+    int r = lane / here, u = lane - r * here;
+    F sum{};
+    while (r < pl.rows) {
+      add_to(sum, red[r * width + lo + u]);
+      r += skip_r;
+      u += skip_u;
+      if (u >= here) {
+        u -= here;
+        ++r;
+      }
+    }
+    sum = over_wave(sum);
+    if (lane == 0) done(g, sum);
+  }
+}
+
+// A thread's sum and sum of squares of its values, per channel, about its
+// first value: a mean far from 0 costs no digits, and a first value far from
+// the others costs no more than it adds to the variance itself.
+template <int V>
+struct Moments {
+  float k[V], s1[V], s2[V];
+  __device__ __forceinline__ void begin() {
+#pragma unroll
+    for (int j = 0; j < V; ++j) k[j] = s1[j] = s2[j] = 0.0f;
+  }
+  __device__ __forceinline__ void about(const float (&v)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) k[j] = v[j];
+  }
+  __device__ __forceinline__ void add(const float (&v)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float d = v[j] - k[j];
+      s1[j] += d;
+      s2[j] = fmaf(d, d, s2[j]);
+    }
+  }
+  // (s1, s2) -> (mean, squares about it) of n values
+  __device__ __forceinline__ void close(float n) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float m = s1[j] / n;
+      s2[j] = fmaxf(s2[j] - s1[j] * m, 0.0f);
+      s1[j] = k[j] + m;
+    }
+  }
+};
+
+// Joins the threads' moments.  Two rounds of sums: first the groups' means,
+// into mean[g]; then what rounding left of them (about the first result,
+// nothing cancels) and the squares about it.  fold(g, mean, squares) is called
+// by one lane per group that has values here, n_of(g) many, and decides what
+// becomes of them.  red: THREADS * units float2.
+template <int V, typename Count, typename Fold>
+__device__ __forceinline__ void join_moments(Moments<V>& t, int count,
+                                             float2* red, float* mean,
+                                             const Place& pl, int c0, int cg,
+                                             int units, Count n_of,
+                                             Fold fold) {
+  const int per = V / units;
+  const int first = c0 / per, upg = cg / per, width = pl.cols * units;
+  const float n = (float)count;
+  float* red1 = reinterpret_cast<float*>(red);
+  float a[V];
+  if (count) t.close(n);
+#pragma unroll
+  for (int j = 0; j < V; ++j) a[j] = n * t.s1[j];
+  if (pl.on) put_units<V>(red1, units, a);
+  __syncthreads();
+  sum_groups(red1, pl, width, first, upg,
+             [&](int g, float sum) { mean[g] = sum / n_of(g); });
+  __syncthreads();
+  if (pl.on) {
+    float2 q[V];
+    each_group<V>(c0 + pl.col * V, cg, [&](int j, int g) {
+      const float e = t.s1[j] - mean[g];
+      q[j] = make_float2(n * e, fmaf(n * e, e, t.s2[j]));
+    });
+    if (count == 0) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) q[j] = make_float2(0.0f, 0.0f);
+    }
+    put_units<V>(red, units, q);
+  }
+  __syncthreads();
+  sum_groups(red, pl, width, first, upg, [&](int g, float2 sum) {
+    const float shift = sum.x / n_of(g);
+    fold(g, mean[g] + shift, fmaxf(sum.y - sum.x * shift, 0.0f));
+  });
+  __syncthreads();
+}
+
+// Sums over the rows of a block, channel by channel.  Threads bring s1 and s2
+// of their V channels; out1[c] and out2[c] (LDS) get the totals of the row's
+// channels.  In rounds of up to 4 channels; red: RED_CHANNELS(V) floats.
+constexpr int ROUND(int v) { return v < 4 ? v : 4; }
+constexpr int RED_CHANNELS(int v) { return THREADS * 2 * ROUND(v); }
+
+template <int V>
+__device__ __forceinline__ void sum_channels(float* red, const Place& pl,
+                                             const float (&s1)[V],
+                                             const float (&s2)[V], float* out1,
+                                             float* out2) {
+  constexpr int R = ROUND(V);
+  const int items = pl.cols * 2 * R;   // sums of a row
+  const int subs = min(THREADS / items, pl.rows);
+  const int sub = threadIdx.x / items, item = threadIdx.x - sub * items;
+#pragma unroll
+  for (int j = 0; j < V; j += R) {
+    auto leave = [&](int i, float t) {
+      const int col = i / (2 * R), q = i % (2 * R);
+      (q < R ? out1 : out2)[col * V + j + q % R] = t;
+    };
+    if (pl.on) {
+      Pack<float, 2 * R> v;
+#pragma unroll
+      for (int q = 0; q < R; ++q) {
+        v.v[q] = s1[j + q];
+        v.v[R + q] = s2[j + q];
+      }
+      store_pack<float, 2 * R>(red + threadIdx.x * 2 * R, v);
+    }
+    __syncthreads();
+    if (subs <= 1) {  // few rows
+      for (int i = threadIdx.x; i < items; i += THREADS) {
+        float t = 0.0f;
+        for (int r = 0; r < pl.rows; ++r) t += red[r * items + i];
+        leave(i, t);
+      }
+    } else {  // a thread sums a share of an item's rows, then the shares
+      float t = 0.0f;
+      if (sub < subs) {
+#pragma unroll 4
+        for (int r = sub; r < pl.rows; r += subs) t += red[r * items + item];
+      }
+      __syncthreads();
+      if (sub < subs) red[threadIdx.x] = t;
+      __syncthreads();
+      if ((int)threadIdx.x < items) {
+        t = 0.0f;
+#pragma unroll 4
+        for (int q = 0; q < subs; ++q) t += red[q * items + threadIdx.x];
+        leave(threadIdx.x, t);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Channel sums s1[c], s2[c] (LDS, channels first .. first + width of C) ->
+// the groups' sums weighted by w; fold(g, s1, s2) is called by one lane.
+template <typename Fold>
+__device__ __forceinline__ void weigh_groups(const float* s1, const float* s2,
+                                             const float* __restrict__ w,
+                                             int first, int width, int cg,
+                                             Fold fold) {
+  const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
+  const int last = first + width;
+  for (int g = first / cg + wave; g * cg < last; g += THREADS / WAVE) {
+    const int lo = max(g * cg, first), hi = min((g + 1) * cg, last);
+    float a = 0.0f, c = 0.0f;
+    for (int i = lo + lane; i < hi; i += WAVE) {
+      const float wi = w ? w[i] : 1.0f;
+      a = fmaf(wi, s1[i - first], a);
+      c = fmaf(wi, s2[i - first], c);
+    }
+    a = wave_sum(a);
+    c = wave_sum(c);
+    if (lane == 0) fold(g, a, c);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// values
+// ---------------------------------------------------------------------------
+// z = (x - m) a + o, per channel of a thread's vector: a = rstd w, o = b.
+// Parameters first: they can be on their way while statistics are not known.
+template <int V>
+struct Affine {
+  float m[V], a[V], o[V];
+  __device__ __forceinline__ void params(int ch, const float* __restrict__ w,
+                                         const float* __restrict__ bias) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      a[j] = w ? w[ch + j] : 1.0f;
+      o[j] = bias ? bias[ch + j] : 0.0f;
+    }
+  }
+  // indexed by group; channel ch is the thread's first
+  __device__ __forceinline__ void stats(int ch, int cg, const float* mean,
+                                        const float* rstd) {
+    each_group<V>(ch, cg, [&](int j, int g) {
+      m[j] = mean[g];
+      a[j] *= rstd[g];
+    });
+  }
+};
+
+template <typename T, int V, int ACT, bool DROP>
+__device__ __forceinline__ Pack<T, V> forward_value(
+    const Affine<V>& k, const Pack<T, V>& raw, int act, const DropoutArgs& d,
+    const DropoutState& st, uint64_t at) {
+  float v[V];
+  unpack<T, V>(raw, v);
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = fmaf(v[j] - k.m[j], k.a[j], k.o[j]);
+  act_apply<T, ACT, V>(act, v);
+  if (DROP && d.on) dropout_apply<V>(d, st, at, v);
+  return pack<T, V>(v);
+}
+
+// (x, gy) -> (x - mean, gz)
+template <typename T, int V, int ACT, bool DROP>
+__device__ __forceinline__ void through(const Affine<V>& k,
+                                        const Pack<T, V>& rx,
+                                        const Pack<T, V>& rg, int act,
+                                        const DropoutArgs& d,
+                                        const DropoutState& st, uint64_t at,
+                                        float (&e)[V], float (&g)[V]) {
+  unpack<T, V>(rx, e);
+  unpack<T, V>(rg, g);
+  float z[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    e[j] -= k.m[j];
+    z[j] = fmaf(e[j], k.a[j], k.o[j]);
+  }
+  act_backward<ACT, V>(act, z, g);
+  if (DROP && d.on) dropout_apply<V>(d, st, at, g);
+}
+
+// ---------------------------------------------------------------------------
+// tile route
+// ---------------------------------------------------------------------------
+struct Tiles {
+  int span, spans;  // channels of a tile, tiles of a sample
+  int groups;       // groups of a tile
+  int iters;        // vectors per thread
+};
+
+// Vectors that a thread asks for at once, of one tensor or of each of two.  All
+// are asked for without a branch (past the end, the last one again): a load
+// under a condition is waited for before the next.
+template <typename T>
+constexpr int AHEAD1 = sizeof(T) == 2 ? 4 : 2;
+template <typename T>
+constexpr int AHEAD2 = sizeof(T) == 2 ? 4 : 2;
+
+// LDS: the tile, red, then floats per group.
+template <typename T, int V, int ACT, bool DROP>
+__global__ __launch_bounds__(THREADS, 4) void gn_tile(
+    const T* __restrict__ x, T* __restrict__ y, const float* __restrict__ w,
+    const float* __restrict__ bias, float* __restrict__ mean_out,
+    float* __restrict__ rstd_out, Shape s, Tiles tiles, int units, float eps,
+    int act, DropoutArgs d) {
+  extern __shared__ char lds[];
+  Pack<T, V>* slots = reinterpret_cast<Pack<T, V>*>(lds);
+  float2* red = reinterpret_cast<float2*>(slots + tiles.iters * THREADS);
+  float* mean = reinterpret_cast<float*>(red + THREADS * units);
+  float* rstd = mean + tiles.groups;
+  const int span = blockIdx.x % tiles.spans, b = blockIdx.x / tiles.spans;
+  const Place pl(tiles.span / V, THREADS);
+  const int ch = span * tiles.span + pl.col * V;  // the thread's first channel
+  const int64_t from = (int64_t)b * s.hw * s.c + ch;
+  const int count = pl.count((int)s.hw);
+
+  auto load = [&](int i) {
+    return load_pack<T, V>(x + from + (int64_t)(pl.row + i * pl.rows) * s.c);
+  };
+  Moments<V> t;
+  t.begin();
+  Affine<V> k;
+  if (count) {
+    constexpr int D = AHEAD1<T>;
+    for (int i = 0; i < count; i += D) {
+      Pack<T, V> raw[D];
+#pragma unroll
+      for (int q = 0; q < D; ++q) raw[q] = load(min(i + q, count - 1));
+      if (i == 0) k.params(ch, w, bias);
+      float v[V];
+      if (i == 0) {
+        unpack<T, V>(raw[0], v);
+        t.about(v);
+      }
+#pragma unroll
+      for (int q = 0; q < D; ++q) {
+        if (i + q >= count) continue;
+        slots[(i + q) * THREADS + threadIdx.x] = raw[q];
+        unpack<T, V>(raw[q], v);
+        t.add(v);
+      }
+    }
+  }
+  const float n = (float)s.hw * (float)s.cg;
+  join_moments<V>(t, count, red, mean, pl, 0, s.cg, units,
+                  [&](int) { return n; },
+                  [&](int g, float m, float m2) {
+                    const float r = rstd_of(m2, n, eps);
+                    mean[g] = m;
+                    rstd[g] = r;
+                    if (mean_out) {
+                      const int64_t at =
+                          (int64_t)b * s.g + span * tiles.groups + g;
+                      mean_out[at] = m;
+                      rstd_out[at] = r;
+                    }
+                  });
+  if (count == 0) return;
+  const DropoutState st = dropout_state(d);
+  k.stats(pl.col * V, s.cg, mean, rstd);
+  for (int i = 0; i < count; ++i) {
+    const int64_t at = from + (int64_t)(pl.row + i * pl.rows) * s.c;
+    store_pack<T, V>(y + at,
+                     forward_value<T, V, ACT, DROP>(
+                         k, slots[i * THREADS + threadIdx.x], act, d, st,
+                         (uint64_t)at));
+  }
+}
+
+// LDS: x's and gy's tiles, red, then floats per channel and per group.
+// sums_c: [2][b][c] of the samples' sums of gz and gz xhat, for the
+// parameters' gradients; null where those are not asked for.
+template <typename T, int V, int ACT, bool DROP>
+__global__ __launch_bounds__(THREADS, 4) void gn_bwd_tile(
+    const T* __restrict__ x, const T* __restrict__ gy, T* __restrict__ dx,
+    const float* __restrict__ w, const float* __restrict__ bias,
+    const float* __restrict__ mean, const float* __restrict__ rstd,
+    float* __restrict__ sums_c, Shape s, Tiles tiles, int act, DropoutArgs d) {
+  extern __shared__ char lds[];
+  Pack<T, V>* slots = reinterpret_cast<Pack<T, V>*>(lds);
+  const int slot_g = tiles.iters * THREADS;  // gy's slots behind x's
+  float* red = reinterpret_cast<float*>(slots + 2 * slot_g);
+  float* sum1 = red + RED_CHANNELS(V);
+  float* sum2 = sum1 + tiles.span;
+  float* t1 = sum2 + tiles.span;
+  float* t2 = t1 + tiles.groups;
+  const int span = blockIdx.x % tiles.spans, b = blockIdx.x / tiles.spans;
+  const Place pl(tiles.span / V, THREADS);
+  const int c0 = span * tiles.span, ch = c0 + pl.col * V;
+  const int64_t from = (int64_t)b * s.hw * s.c + ch;
+  const int count = pl.count((int)s.hw);
+  const DropoutState st = dropout_state(d);
+  mean += (int64_t)b * s.g;
+  rstd += (int64_t)b * s.g;
+  Affine<V> k;
+
+  float s1[V], s2[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0f;
+  auto place = [&](int i) {
+    return from + (int64_t)(pl.row + i * pl.rows) * s.c;
+  };
+  if (count) {
+    constexpr int D = AHEAD2<T> / 2;
+    k.params(ch, w, bias);
+    k.stats(ch, s.cg, mean, rstd);
+    for (int i = 0; i < count; i += D) {
+      Pack<T, V> rx[D], rg[D];
+#pragma unroll
+      for (int q = 0; q < D; ++q) {
+        const int64_t at = place(min(i + q, count - 1));
+        rx[q] = load_pack<T, V>(x + at);
+        rg[q] = load_pack<T, V>(gy + at);
+      }
+#pragma unroll
+      for (int q = 0; q < D; ++q) {
+        if (i + q >= count) continue;
+        slots[(i + q) * THREADS + threadIdx.x] = rx[q];
+        slots[slot_g + (i + q) * THREADS + threadIdx.x] = rg[q];
+        float e[V], g[V];
+        through<T, V, ACT, DROP>(k, rx[q], rg[q], act, d, st,
+                                 (uint64_t)place(i + q), e, g);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          s1[j] += g[j];
+          s2[j] = fmaf(g[j], e[j], s2[j]);
+        }
+      }
+    }
+  }
+  if (count)
+    each_group<V>(ch, s.cg, [&](int j, int g) { s2[j] *= rstd[g]; });
+  sum_channels<V>(red, pl, s1, s2, sum1, sum2);
+  const float inv_n = 1.0f / ((float)s.hw * (float)s.cg);
+  weigh_groups(sum1, sum2, w, c0, tiles.span, s.cg,
+               [&](int g, float a, float c) {
+                 const float r = rstd[g];
+                 t1[g - span * tiles.groups] = -r * (a * inv_n);
+                 t2[g - span * tiles.groups] = -r * r * (c * inv_n);
+               });
+  if (sums_c)
+    for (int c = threadIdx.x; c < tiles.span; c += THREADS) {
+      sums_c[(int64_t)b * s.c + c0 + c] = sum1[c];
+      sums_c[((int64_t)s.b + b) * s.c + c0 + c] = sum2[c];
+    }
+  if (!dx) return;
+  __syncthreads();
+  if (count == 0) return;
+  float m1[V], m2[V];
+  each_group<V>(pl.col * V, s.cg, [&](int j, int g) {
+    m1[j] = t1[g];
+    m2[j] = t2[g];
+  });
+  for (int i = 0; i < count; ++i) {
+    const int64_t at = from + (int64_t)(pl.row + i * pl.rows) * s.c;
+    float e[V], g[V];
+    through<T, V, ACT, DROP>(k, slots[i * THREADS + threadIdx.x],
+                       slots[slot_g + i * THREADS + threadIdx.x], act, d, st,
+                       (uint64_t)at, e, g);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      g[j] = fmaf(k.a[j], g[j], fmaf(e[j], m2[j], m1[j]));
+    store_pack<T, V>(dx + at, pack<T, V>(g));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// split route
+// ---------------------------------------------------------------------------
+// Block (split, sample).  part: [b][g][splits] of (mean, M2); n follows from
+// the split's bounds.  Rows wider than a block are taken in chunks of columns,
+// and groups that reach over chunks are joined as they come.
+template <typename T, int V>
+__global__ __launch_bounds__(THREADS, 4) void gn_stats(
+    const T* __restrict__ x, float2* __restrict__ part, Shape s, Cut cut,
+    int units) {
+  constexpr int D = AHEAD1<T>;
+  __shared__ float2 red[THREADS * V];
+  extern __shared__ float joined[];  // [4][g]: work space, then n, mean, M2
+  float* mean = joined;
+  float* jn = mean + s.g;
+  float* jm = jn + s.g;
+  float* jq = jm + s.g;
+  const int split = blockIdx.x % cut.n, b = blockIdx.x / cut.n;
+  const int pixels = cut.pixels(split);
+  const T* base = x + ((int64_t)b * s.hw + cut.first(split)) * s.c;
+  for (int c0 = 0; c0 < s.c; c0 += THREADS * V) {
+    const Place pl(min(THREADS, (s.c - c0) / V), THREADS);
+    const int count = pl.count(pixels);
+    const int64_t next = (int64_t)pl.rows * s.c;
+    const T* at = base + (int64_t)pl.row * s.c + c0 + pl.col * V;
+    Moments<V> t;
+    t.begin();
+    for (int i = 0; i < count; i += D) {
+      Pack<T, V> raw[D];
+#pragma unroll
+      for (int q = 0; q < D; ++q)
+        raw[q] = load_pack<T, V>(at + min(i + q, count - 1) * next);
+      float v[V];
+      if (i == 0) {
+        unpack<T, V>(raw[0], v);
+        t.about(v);
+      }
+#pragma unroll
+      for (int q = 0; q < D; ++q) {
+        if (i + q >= count) continue;
+        unpack<T, V>(raw[q], v);
+        t.add(v);
+      }
+    }
+    const int last = c0 + pl.cols * V;
+    // values of group g in this chunk
+    auto n_of = [&](int g) {
+      return (float)(min((g + 1) * s.cg, last) - max(g * s.cg, c0)) *
+             (float)pixels;
+    };
+    join_moments<V>(t, count, red, mean, pl, c0, s.cg, units, n_of,
+                    [&](int g, float m, float q) {
+                      float n = n_of(g);
+                      if (g * s.cg < c0) {  // begun in an earlier chunk
+                        const float d = m - jm[g], sum = jn[g] + n;
+                        q += jq[g] + d * d * (jn[g] * n / sum);
+                        m = jm[g] + d * (n / sum);
+                        n = sum;
+                      }
+                      jn[g] = n;
+                      jm[g] = m;
+                      jq[g] = q;
+                    });
+  }
+  for (int g = threadIdx.x; g < s.g; g += THREADS)
+    part[((int64_t)b * s.g + g) * cut.n + split] = make_float2(jm[g], jq[g]);
+}
+
+// `lanes` neighbouring threads, a power of two and at most a wave, share a
+// group and take every lanes-th of its partial sums, MOST at a time.
+constexpr int MOST = 8;
+
+struct Share {
+  int lanes, lane, group, step;
+  __device__ __forceinline__ explicit Share(int groups) {
+    lanes = WAVE;
+    while (lanes > 1 && lanes * groups > THREADS) lanes >>= 1;
+    lane = threadIdx.x & (lanes - 1);
+    group = threadIdx.x / lanes;
+    step = THREADS / lanes;
+  }
+  __device__ __forceinline__ float sum(float v) const {
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, WAVE);
+    return v;
+  }
+  // f(i, entry) over this thread's entries below n
+  template <typename F>
+  __device__ __forceinline__ void each(const float2* e, int n, F f) const {
+    for (int i = lane; i < n; i += MOST * lanes) {
+      float2 v[MOST];
+#pragma unroll
+      for (int q = 0; q < MOST; ++q)
+        if (i + q * lanes < n) v[q] = e[i + q * lanes];
+#pragma unroll
+      for (int q = 0; q < MOST; ++q)
+        if (i + q * lanes < n) f(i + q * lanes, v[q]);
+    }
+  }
+};
+
+// A block per sample: joins the splits' statistics, the mean first, about
+// split 0's, then squares about it.  stat: [2][b][g] mean and rstd.
+__global__ __launch_bounds__(THREADS) void gn_join(
+    const float2* __restrict__ part, float* __restrict__ stat, Shape s,
+    Cut cut, float eps) {
+  const int b = blockIdx.x;
+  const Share sh(s.g);
+  for (int g = sh.group; g < s.g; g += sh.step) {
+    const float2* e = part + ((int64_t)b * s.g + g) * cut.n;
+    const float ref = e[0].x;
+    float sm = 0.0f, sq = 0.0f;
+    sh.each(e, cut.n, [&](int i, float2 v) {
+      sm += (float)cut.pixels(i) * (v.x - ref);
+    });
+    const float mean = ref + sh.sum(sm) / (float)s.hw;
+    sh.each(e, cut.n, [&](int i, float2 v) {
+      const float d = v.x - mean;
+      sq += fmaf((float)cut.pixels(i) * (float)s.cg, d * d, v.y);
+    });
+    sq = sh.sum(sq);
+    if (sh.lane == 0) {
+      stat[(int64_t)b * s.g + g] = mean;
+      stat[((int64_t)s.b + b) * s.g + g] =
+          rstd_of(sq, (float)s.hw * (float)s.cg, eps);
+    }
+  }
+}
+
+// Block (sample, piece of pixels, chunk of columns).  Pieces are short and in
+// memory's order: blocks that run together then read and write neighbouring
+// memory (403 MB copied in 145 us; by 2048 blocks, each with a long piece of
+// its own, in 166 us).
+struct Pieces {
+  int pixels, pieces, chunks;  // pixels of a piece; pieces, column chunks
+};
+
+template <typename T, int V, int ACT, bool DROP>
+__global__ __launch_bounds__(BLOCK) void gn_apply(
+    const T* __restrict__ x, T* __restrict__ y, const float* __restrict__ w,
+    const float* __restrict__ bias, const float* __restrict__ stat, Shape s,
+    Pieces ps, bool stream, int act, DropoutArgs d) {
+  const int chunk = blockIdx.x % ps.chunks, rest = blockIdx.x / ps.chunks;
+  const int piece = rest % ps.pieces, b = rest / ps.pieces;
+  const int c0 = chunk * BLOCK * V;
+  const Place pl(min(BLOCK, (s.c - c0) / V), BLOCK);
+  const int64_t first = (int64_t)piece * ps.pixels;
+  const int count = pl.count((int)min((int64_t)ps.pixels, s.hw - first));
+  if (count == 0) return;
+  const int ch = c0 + pl.col * V;
+  const int64_t from = ((int64_t)b * s.hw + first + pl.row) * s.c + ch;
+  const int64_t next = (int64_t)pl.rows * s.c;
+  const DropoutState st = dropout_state(d);
+  constexpr int D = AHEAD1<T>;
+  Affine<V> k;
+  k.params(ch, w, bias);
+  k.stats(ch, s.cg, stat + (int64_t)b * s.g, stat + ((int64_t)s.b + b) * s.g);
+  for (int i = 0; i < count; i += D) {
+    Pack<T, V> raw[D];
+#pragma unroll
+    for (int q = 0; q < D; ++q)
+      raw[q] = load_pack<T, V>(x + from + min(i + q, count - 1) * next, stream);
+#pragma unroll
+    for (int q = 0; q < D; ++q) {
+      if (i + q >= count) continue;
+      const int64_t at = from + (i + q) * next;
+      store_pack<T, V>(y + at,
+                       forward_value<T, V, ACT, DROP>(k, raw[q], act, d, st,
+                                                      (uint64_t)at),
+                       stream);
+    }
+  }
+}
+
+// Block (split, sample): sums of gz and gz xhat of every channel over the
+// split's pixels.  part_c: [2][b * splits][c]; part_g: [b][g][splits] of the
+// same sums weighted by w and added up over the group.
+template <typename T, int V, int ACT, bool DROP>
+__global__ __launch_bounds__(THREADS, 4) void gn_bwd_sums(
+    const T* __restrict__ x, const T* __restrict__ gy,
+    const float* __restrict__ w, const float* __restrict__ bias,
+    const float* __restrict__ stat, float* __restrict__ part_c,
+    float2* __restrict__ part_g, Shape s, Cut cut, int act, DropoutArgs d) {
+  extern __shared__ float lds_sums[];  // red; [2][channels]; [2][g]
+  float* red = lds_sums;
+  float* sum1 = red + RED_CHANNELS(V);
+  float* sum2 = sum1 + min(THREADS * V, s.c);
+  float* joined = sum2 + min(THREADS * V, s.c);
+  const int split = blockIdx.x % cut.n, b = blockIdx.x / cut.n;
+  const DropoutState st = dropout_state(d);
+  const int pixels = cut.pixels(split);
+  const int64_t from = ((int64_t)b * s.hw + cut.first(split)) * s.c;
+  const float* mean = stat + (int64_t)b * s.g;
+  const float* rstd = stat + ((int64_t)s.b + b) * s.g;
+  float* out1 = part_c + ((int64_t)b * cut.n + split) * s.c;
+  float* out2 = out1 + (int64_t)s.b * cut.n * s.c;
+  for (int c0 = 0; c0 < s.c; c0 += THREADS * V) {
+    const Place pl(min(THREADS, (s.c - c0) / V), THREADS);
+    const int count = pl.count(pixels);
+    const int64_t next = (int64_t)pl.rows * s.c;
+    const int ch = c0 + pl.col * V;
+    const int64_t at = from + (int64_t)pl.row * s.c + ch;
+    float s1[V], s2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0f;
+    if (count) {
+      constexpr int D = AHEAD2<T>;
+      Affine<V> k;
+      k.params(ch, w, bias);
+      k.stats(ch, s.cg, mean, rstd);
+      for (int i = 0; i < count; i += D) {
+        Pack<T, V> rx[D], rg[D];
+#pragma unroll
+        for (int q = 0; q < D; ++q) {
+          const int64_t to = at + min(i + q, count - 1) * next;
+          rx[q] = load_pack<T, V>(x + to);
+          rg[q] = load_pack<T, V>(gy + to);
+        }
+#pragma unroll
+        for (int q = 0; q < D; ++q) {
+          if (i + q >= count) continue;
+          float e[V], g[V];
+          through<T, V, ACT, DROP>(k, rx[q], rg[q], act, d, st,
+                                   (uint64_t)(at + (i + q) * next), e, g);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            s1[j] += g[j];
+            s2[j] = fmaf(g[j], e[j], s2[j]);
+          }
+        }
+      }
+    }
+    if (count)
+      each_group<V>(ch, s.cg, [&](int j, int g) { s2[j] *= rstd[g]; });
+    sum_channels<V>(red, pl, s1, s2, sum1, sum2);
+    const int width = pl.cols * V;
+    for (int c = threadIdx.x; c < width; c += THREADS) {
+      out1[c0 + c] = sum1[c];
+      out2[c0 + c] = sum2[c];
+    }
+    weigh_groups(sum1, sum2, w, c0, width, s.cg, [&](int g, float a, float c) {
+      const bool begun = g * s.cg < c0;
+      joined[g] = a + (begun ? joined[g] : 0.0f);
+      joined[s.g + g] = c + (begun ? joined[s.g + g] : 0.0f);
+    });
+    __syncthreads();
+  }
+  for (int g = threadIdx.x; g < s.g; g += THREADS)
+    part_g[((int64_t)b * s.g + g) * cut.n + split] =
+        make_float2(joined[g], joined[s.g + g]);
+}
+
+// A block per sample: coef, [2][b][g], gets what dx adds to rstd w gz:
+// coef0 + (x - mean) coef1.
+__global__ __launch_bounds__(THREADS) void gn_bwd_join(
+    const float2* __restrict__ part_g, const float* __restrict__ stat,
+    float* __restrict__ coef, Shape s, Cut cut) {
+  const int b = blockIdx.x;
+  const Share sh(s.g);
+  const float inv_n = 1.0f / ((float)s.hw * (float)s.cg);
+  for (int g = sh.group; g < s.g; g += sh.step) {
+    float a = 0.0f, c = 0.0f;
+    sh.each(part_g + ((int64_t)b * s.g + g) * cut.n, cut.n,
+            [&](int, float2 v) {
+              a += v.x;
+              c += v.y;
+            });
+    a = sh.sum(a);
+    c = sh.sum(c);
+    if (sh.lane == 0) {
+      const float r = stat[((int64_t)s.b + b) * s.g + g];
+      coef[(int64_t)b * s.g + g] = -r * (a * inv_n);
+      coef[((int64_t)s.b + b) * s.g + g] = -r * r * (c * inv_n);
+    }
+  }
+}
+
+// Channels [8 block, 8 block + 8): sums of `rows` rows of part ([2][rows][c])
+// into db and dw (either may be null).
+__device__ __forceinline__ void param_sums(const float* __restrict__ part,
+                                           int64_t rows, int c, int block,
+                                           float* __restrict__ db,
+                                           float* __restrict__ dw,
+                                           float* red /* [BLOCK] */) {
+  const int ch = block * 8 + (threadIdx.x & 7);
+  const int r0 = threadIdx.x >> 3;
+  for (int which = 0; which < 2; ++which) {
+    float* out = which ? dw : db;
+    if (!out) continue;
+    const float* at = part + (int64_t)which * rows * c + ch;
+    float sum = 0.0f;
+    if (ch < c) {
+#pragma unroll 8
+      for (int64_t r = r0; r < rows; r += BLOCK / 8) sum += at[r * c];
+    }
+    red[threadIdx.x] = sum;
+    __syncthreads();
+    if (threadIdx.x < 8 && ch < c) {
+      float total = 0.0f;
+      for (int i = 0; i < BLOCK / 8; ++i) total += red[i * 8 + threadIdx.x];
+      out[ch] = total;
+    }
+    __syncthreads();
+  }
+}
+
+__global__ __launch_bounds__(BLOCK) void gn_param_grad(
+    const float* __restrict__ part, int64_t rows, int c,
+    float* __restrict__ db, float* __restrict__ dw) {
+  __shared__ float red[BLOCK];
+  param_sums(part, rows, c, blockIdx.x, db, dw, red);
+}
+
+// The first `param_blocks` blocks sum the parameters' gradients while the
+// others, laid out as gn_apply's, write dx.
+template <typename T, int V, int ACT, bool DROP>
+__global__ __launch_bounds__(BLOCK, 4) void gn_bwd_dx(
+    const T* __restrict__ x, const T* __restrict__ gy, T* __restrict__ dx,
+    const float* __restrict__ w, const float* __restrict__ bias,
+    const float* __restrict__ stat, const float* __restrict__ coef,
+    const float* __restrict__ part_c, int64_t part_rows,
+    float* __restrict__ db, float* __restrict__ dw, Shape s, Pieces ps,
+    int param_blocks, bool stream, int act, DropoutArgs d) {
+  __shared__ float red[BLOCK];
+  if ((int)blockIdx.x < param_blocks) {
+    param_sums(part_c, part_rows, s.c, blockIdx.x, db, dw, red);
+    return;
+  }
+  const int block = blockIdx.x - param_blocks;
+  const int chunk = block % ps.chunks, rest = block / ps.chunks;
+  const int piece = rest % ps.pieces, b = rest / ps.pieces;
+  const int c0 = chunk * BLOCK * V;
+  const Place pl(min(BLOCK, (s.c - c0) / V), BLOCK);
+  const int64_t first = (int64_t)piece * ps.pixels;
+  const int count = pl.count((int)min((int64_t)ps.pixels, s.hw - first));
+  if (count == 0) return;
+  const int ch = c0 + pl.col * V;
+  const int64_t from = ((int64_t)b * s.hw + first + pl.row) * s.c + ch;
+  const int64_t next = (int64_t)pl.rows * s.c;
+  const DropoutState st = dropout_state(d);
+  Affine<V> k;
+  float m1[V], m2[V];
+  auto emit = [&](const Pack<T, V>& rx, const Pack<T, V>& rg, int64_t at) {
+    float e[V], g[V];
+    through<T, V, ACT, DROP>(k, rx, rg, act, d, st, (uint64_t)at, e, g);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      g[j] = fmaf(k.a[j], g[j], fmaf(e[j], m2[j], m1[j]));
+    store_pack<T, V>(dx + at, pack<T, V>(g), stream);
+  };
+  constexpr int D = AHEAD2<T>;
+  k.params(ch, w, bias);
+  k.stats(ch, s.cg, stat + (int64_t)b * s.g, stat + ((int64_t)s.b + b) * s.g);
+  const float* c0s = coef + (int64_t)b * s.g;
+  const float* c1s = c0s + (int64_t)s.b * s.g;
+  each_group<V>(ch, s.cg, [&](int j, int g) {
+    m1[j] = c0s[g];
+    m2[j] = c1s[g];
+  });
+  for (int i = 0; i < count; i += D) {
+    Pack<T, V> rx[D], rg[D];
+#pragma unroll
+    for (int q = 0; q < D; ++q) {
+      const int64_t at = from + min(i + q, count - 1) * next;
+      rx[q] = load_pack<T, V>(x + at, stream);
+      rg[q] = load_pack<T, V>(gy + at, stream);
+    }
+#pragma unroll
+    for (int q = 0; q < D; ++q)
+      if (i + q < count) emit(rx[q], rg[q], from + (i + q) * next);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+bool aligned(const void* p, size_t to) {
+  return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0;
+}
+
+// Channels a thread moves at once: the most of 8, 4 and 1 that divide C and
+// whose vectors are aligned.
+template <typename T>
+int vector_of(const Shape& s, std::initializer_list<const void*> ptrs) {
+  for (int v : {8, 4}) {
+    const size_t to = std::min<size_t>(16, v * sizeof(T));
+    bool ok = s.c % v == 0;
+    for (const void* p : ptrs) ok = ok && aligned(p, to);
+    if (ok) return v;
+  }
+  return 1;
+}
+
+struct Plan {
+  bool tiled;
+  Tiles tiles;
+  int units;  // groups that a vector touches, at most
+  size_t lds;
+};
+
+// LDS of a tile's block: half of a CU's 160 KB, so that one block reads while
+// another writes.
+constexpr size_t TILE_LDS = 80 * 1024;
+
+// How to tile, or that it does not fit.  Spans are multiples of whole groups
+// and whole vectors, of 32 bytes or more where they can be, and wider while
+// that leaves four blocks per CU.
+Plan plan_tiles(const Shape& s, int v, size_t value, bool back) {
+  Plan p{};
+  p.units = v / std::gcd(v, s.cg);
+  const int64_t base = std::lcm((int64_t)s.cg, (int64_t)v);
+  const int64_t widest = std::min<int64_t>(s.c, (int64_t)THREADS * v);
+  const int64_t many = s.c / base;
+  for (int64_t m = 1; m <= many && base * m <= widest; ++m) {
+    if (many % m) continue;
+    const int64_t span = base * m, spans = s.c / span;
+    if (p.tiled && (int64_t)p.tiles.span * (int64_t)value >= 32 &&
+        s.b * spans < 1024)
+      break;
+    const int64_t rows = THREADS / (span / v);
+    const int64_t iters = (s.hw + rows - 1) / rows;
+    const int64_t lds =
+        iters * THREADS * v * (int64_t)value * (back ? 2 : 1) +
+        (back ? 4 * RED_CHANNELS(v) + 8 * span : 8 * THREADS * p.units) +
+        8 * (span / s.cg);
+    if (lds > (int64_t)TILE_LDS) break;
+    if (s.b * spans >= (1ll << 31)) continue;
+    p.tiled = true;
+    p.lds = (size_t)lds;
+    p.tiles = {(int)span, (int)spans, (int)(span / s.cg), (int)iters};
+  }
+  return p;
+}
+
+// Blocks per sample that sum: about 1024 over the batch, each with 16384
+// values or more; at most 256, which a join still reads at once.
+Cut cut_pixels(const Shape& s) {
+  int64_t n = (1024 + s.b - 1) / s.b;
+  n = std::min<int64_t>(n, s.hw * s.c / 16384);
+  n = std::max<int64_t>(1, std::min<int64_t>({n, s.hw, 256}));
+  TORCH_CHECK(s.b * n < (1ll << 31), "group_norm: tensor too large");
+  return {(int)n, (int)(s.hw / n), (int)(s.hw % n)};
+}
+
+// Pieces of `deep` vectors per thread.
+Pieces cut_pieces(const Shape& s, int v, int deep, int64_t more) {
+  const int cols = std::min(BLOCK, s.c / v);
+  Pieces p;
+  p.pixels = BLOCK / cols * deep;
+  p.chunks = (s.c / v + BLOCK - 1) / BLOCK;
+  p.pieces = (int)((s.hw + p.pixels - 1) / p.pixels);
+  TORCH_CHECK((int64_t)s.b * p.pieces * p.chunks + more < (1ll << 31),
+              "group_norm: tensor too large");
+  return p;
+}
+
+// Activations, and whether there is dropout, are compiled in for whole vectors;
+// narrower ones, which odd channel counts take, choose as they go.
+#define GN_ACT(DROP_, ACT_, ...)                \
+  {                                             \
+    constexpr int V = 8, ACT = ACT_;            \
+    constexpr bool DROP = DROP_;                \
+    __VA_ARGS__;                                \
+    break;                                      \
+  }
+#define GN_ACTS(DROP_, ACT_, ...)                            \
+  switch (ACT_) {                                            \
+    case ACT_ELU: GN_ACT(DROP_, ACT_ELU, __VA_ARGS__)        \
+    case ACT_LEAKY: GN_ACT(DROP_, ACT_LEAKY, __VA_ARGS__)    \
+    case ACT_RELU: GN_ACT(DROP_, ACT_RELU, __VA_ARGS__)      \
+    case ACT_SILU: GN_ACT(DROP_, ACT_SILU, __VA_ARGS__)      \
+    default: GN_ACT(DROP_, ACT_NONE, __VA_ARGS__)            \
+  }
+#define GN_VARIANT(V_, ACT_, ON_, ...)          \
+  do {                                          \
+    if (V_ == 8 && ON_) {                       \
+      GN_ACTS(true, ACT_, __VA_ARGS__)          \
+    } else if (V_ == 8) {                       \
+      GN_ACTS(false, ACT_, __VA_ARGS__)         \
+    } else if (V_ == 4) {                       \
+      constexpr int V = 4, ACT = ACT_ANY;       \
+      constexpr bool DROP = true;               \
+      __VA_ARGS__;                              \
+    } else {                                    \
+      constexpr int V = 1, ACT = ACT_ANY;       \
+      constexpr bool DROP = true;               \
+      __VA_ARGS__;                              \
+    }                                           \
+  } while (0)
+
+// More LDS than a launch may ask for without saying so.
+template <typename K>
+void allow_lds(K kernel, size_t bytes) {
+  if (bytes > 64 * 1024)
+    C10_HIP_CHECK(hipFuncSetAttribute(
+        reinterpret_cast<const void*>(kernel),
+        hipFuncAttributeMaxDynamicSharedMemorySize, (int)TILE_LDS));
+}
+
+// stat: [2][b][g] mean and rstd, left for the way back; null: not kept.
+template <typename T>
+void gn_forward(const at::Tensor& x, at::Tensor& y, const float* w,
+             const float* bias, float* stat, const Shape& s, float eps, int act,
+             const DropoutArgs& d) {
+  const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
+  const T* px = (const T*)x.data_ptr();
+  T* py = (T*)y.data_ptr();
+  const int v = vector_of<T>(s, {px, py});
+  const Plan p = plan_tiles(s, v, sizeof(T), false);
+  if (p.tiled) {
+    GN_VARIANT(v, act, d.on, {
+      auto kernel = gn_tile<T, V, ACT, DROP>;
+      allow_lds(kernel, p.lds);
+      hipLaunchKernelGGL(kernel, dim3(s.b * p.tiles.spans), dim3(THREADS),
+                         p.lds, stream, px, py, w, bias, stat, stat ? stat +
+                         (int64_t)s.b * s.g : nullptr, s, p.tiles, p.units,
+                         eps, act, d);
+      C10_HIP_KERNEL_LAUNCH_CHECK();
+    });
+    return;
+  }
+  const Cut cut = cut_pixels(s);
+  const Pieces ps = cut_pieces(s, v, 8, 0);
+  auto buf = at::empty({(int64_t)s.b * s.g * (2 * cut.n + 2)},
+                       x.options().dtype(at::kFloat));
+  float2* part = (float2*)buf.data_ptr();
+  if (!stat) stat = (float*)(part + (int64_t)s.b * s.g * cut.n);
+  const auto stats = v == 8   ? gn_stats<T, 8>
+                     : v == 4 ? gn_stats<T, 4>
+                              : gn_stats<T, 1>;
+  const size_t lds = 4 * (size_t)s.g * 4;
+  allow_lds(stats, lds + THREADS * v * 8);
+  hipLaunchKernelGGL(stats, dim3(s.b * cut.n), dim3(THREADS), lds, stream, px,
+                     part, s, cut, p.units);
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  hipLaunchKernelGGL(gn_join, dim3(s.b), dim3(THREADS), 0, stream, part, stat,
+                     s, cut, eps);
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  const bool nt = x.numel() * (int64_t)sizeof(T) > STREAM_BYTES;
+  GN_VARIANT(v, act, d.on, {
+    hipLaunchKernelGGL((gn_apply<T, V, ACT, DROP>), dim3(s.b * ps.pieces *
+                       ps.chunks), dim3(BLOCK), 0, stream, px, py, w, bias,
+                       stat, s, ps, nt, act, d);
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+  });
+}
+
+template <typename T>
+void gn_backward(const at::Tensor& x, const at::Tensor& gy, at::Tensor& dx_out,
+                 const float* w, const float* bias, const float* stat, float* db, float* dw,
+              const Shape& s, int act, const DropoutArgs& d) {
+  const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
+  const T* px = (const T*)x.data_ptr();
+  const T* pg = (const T*)gy.data_ptr();
+  T* dx = dx_out.defined() ? (T*)dx_out.data_ptr() : nullptr;
+  const int v = vector_of<T>(s, {px, pg, dx});
+  const auto opts = x.options().dtype(at::kFloat);
+  const int param_blocks = db || dw ? (s.c + 7) / 8 : 0;
+  const Plan p = plan_tiles(s, v, sizeof(T), true);
+  if (p.tiled) {
+    at::Tensor buf;
+    float* sums = nullptr;
+    if (param_blocks) {
+      buf = at::empty({2 * (int64_t)s.b * s.c}, opts);
+      sums = buf.data_ptr<float>();
+    }
+    GN_VARIANT(v, act, d.on, {
+      auto kernel = gn_bwd_tile<T, V, ACT, DROP>;
+      allow_lds(kernel, p.lds);
+      hipLaunchKernelGGL(kernel, dim3(s.b * p.tiles.spans), dim3(THREADS),
+                         p.lds, stream, px, pg, dx, w, bias, stat, stat +
+                         (int64_t)s.b * s.g, sums, s, p.tiles, act, d);
+      C10_HIP_KERNEL_LAUNCH_CHECK();
+    });
+    if (param_blocks) {
+      hipLaunchKernelGGL(gn_param_grad, dim3(param_blocks), dim3(BLOCK), 0,
+                         stream, sums, s.b, s.c, db, dw);
+      C10_HIP_KERNEL_LAUNCH_CHECK();
+    }
+    return;
+  }
+  const Cut cut = cut_pixels(s);
+  const Pieces ps = cut_pieces(s, v, 4, param_blocks);
+  const int64_t rows = (int64_t)s.b * cut.n;
+  auto buf = at::empty({2 * rows * (s.c + s.g) + 2 * (int64_t)s.b * s.g}, opts);
+  float2* part_g = (float2*)buf.data_ptr();
+  float* part_c = (float*)(part_g + rows * s.g);
+  float* coef = part_c + 2 * rows * s.c;
+  const bool nt = x.numel() * (int64_t)sizeof(T) > STREAM_BYTES;
+  GN_VARIANT(v, act, d.on, {
+    auto sums = gn_bwd_sums<T, V, ACT, DROP>;
+    const size_t lds =
+        4 * (RED_CHANNELS(V) + 2 * (size_t)std::min(THREADS * V, s.c) + 2 * s.g);
+    allow_lds(sums, lds);
+    hipLaunchKernelGGL(sums, dim3(s.b * cut.n), dim3(THREADS), lds, stream, px,
+                       pg, w, bias, stat, part_c, part_g, s, cut, act, d);
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+    if (dx) {
+      hipLaunchKernelGGL(gn_bwd_join, dim3(s.b), dim3(THREADS), 0, stream,
+                         part_g, stat, coef, s, cut);
+      C10_HIP_KERNEL_LAUNCH_CHECK();
+      hipLaunchKernelGGL((gn_bwd_dx<T, V, ACT, DROP>), dim3(s.b * ps.pieces *
+                         ps.chunks + param_blocks), dim3(BLOCK), 0, stream, px,
+                         pg, dx, w, bias, stat, coef, part_c, rows, db, dw, s,
+                         ps, param_blocks, nt, act, d);
+    } else {
+      hipLaunchKernelGGL(gn_param_grad, dim3(param_blocks), dim3(BLOCK), 0,
+                         stream, part_c, rows, s.c, db, dw);
+    }
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+  });
+}
+
+}  // namespace

@@ -10,22 +10,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-// Element i = 8 j + s has a 32-bit number u(i).  Its upper half is the s-th
-// 16 bits of Philox(key = seed, counter = (j, offset)); its lower half is the
-// same of the counter with bit 63 of j set.  The element is dropped iff
-// u(i) < threshold.  The upper half alone decides unless it equals the
-// threshold's, for one element in 65536, so that 8 elements cost one Philox
-// and yet p is held to 2^-32; where the threshold's lower half is 0 (p = 0.5,
-// 0.25, ...) nothing is ever undecided.
-struct DropoutArgs {
-  const int64_t* rng;   // device [seed, offset], or null: the two below
-  uint64_t seed;
-  uint64_t offset;
-  uint32_t thr_hi;      // threshold's halves; thr_hi = 65536 drops all
-  uint32_t thr_lo;
-  float scale;          // 1 / (1 - p)
-  bool on;
-};
+#include "dropout_args.h"
 
 struct DropoutState {
   uint32_t k0, k1, o0, o1;

@@ -6,6 +6,7 @@ The .so lands in deepof_amd/ops/hip/ so it travels with the repo
 snapshot to GPU boxes (no JIT cache dependence).
 """
 
+import glob
 import os
 
 os.environ.setdefault("PYTORCH_ROCM_ARCH", "gfx950")
@@ -16,6 +17,13 @@ from torch.utils.cpp_extension import BuildExtension, CUDAExtension
 ROOT = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join("deepof_amd", "ops", "hip")
 
+# the generated build file does not know which headers an object was built
+# from: objects older than a header are built again
+newest = max(os.path.getmtime(h) for h in glob.glob(os.path.join(ROOT, SRC, "*.h")))
+for obj in glob.glob(os.path.join(ROOT, "build", "temp.*", SRC, "*.o")):
+    if os.path.getmtime(obj) < newest:
+        os.remove(obj)
+
 ext = CUDAExtension(
     name="deepof_amd.ops.hip._deepof_hip",
     sources=[
@@ -25,8 +33,12 @@ ext = CUDAExtension(
         os.path.join(SRC, "adam.hip"),
         os.path.join(SRC, "conv_mfma.hip"),
         os.path.join(SRC, "conv_wrw2.hip"),
-        os.path.join(SRC, "group_norm.hip"),
+        os.path.join(SRC, "group_norm.cpp"),
+        os.path.join(SRC, "group_norm_f32.hip"),
+        os.path.join(SRC, "group_norm_f16.hip"),
+        os.path.join(SRC, "group_norm_bf16.hip"),
         os.path.join(SRC, "dropout.hip"),
+        os.path.join(SRC, "autograd.cpp"),
     ],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
