@@ -59,7 +59,7 @@ __global__ __launch_bounds__(BLOCK) void dropout_kernel(
       if (need_x) {
         float z[8];
         unpack<T, 8>(rx[i], z);
-        act_backward<ACT, 8>(act, z, v);
+        act_backward<T, ACT, 8>(act, z, v);
       }
     } else {
       unpack<T, 8>(rx[i], v);

@@ -17,7 +17,7 @@ GroupNormShape shape_of(const at::Tensor& x, int64_t groups) {
                   x.size(1) % groups == 0,
               "group_norm: the channels must divide into 1 to ", MAX_GROUPS,
               " groups");
-  TORCH_CHECK(x.size(0) < (1ll << 24) && x.size(1) < (1ll << 24) &&
+  TORCH_CHECK(x.size(0) < (1ll << 24) && x.size(1) < (1ll << 20) &&
                   x.size(2) * x.size(3) < (1ll << 30),
               "group_norm: tensor too large");
   GroupNormShape s;
@@ -29,14 +29,18 @@ GroupNormShape shape_of(const at::Tensor& x, int64_t groups) {
   return s;
 }
 
-const float* param(const at::Tensor& t, const at::Tensor& x,
-                   const char* name) {
-  if (!t.defined()) return nullptr;
+// The parameter, checked, where vectors of 4 can be read from it.
+at::Tensor param(const at::Tensor& t, const at::Tensor& x, const char* name) {
+  if (!t.defined()) return t;
   TORCH_CHECK(t.scalar_type() == at::kFloat && t.is_contiguous() &&
                   t.dim() == 1 && t.size(0) == x.size(1) &&
                   t.device() == x.device(),
               "group_norm: ", name, " must be C floats on the input's device");
-  return t.data_ptr<float>();
+  return (uintptr_t)t.data_ptr() % 16 ? t.clone() : t;
+}
+
+const float* pointer(const at::Tensor& t) {
+  return t.defined() ? t.data_ptr<float>() : nullptr;
 }
 
 #define GN_TYPE(t, call, args)                                              \
@@ -60,8 +64,8 @@ std::vector<at::Tensor> group_norm_forward(
   TORCH_CHECK(eps > 0.0, "group_norm: eps must be positive");
   c10::DeviceGuard guard(x.device());
   const DropoutArgs d = dropout_args(p, rng, seed, offset, x);
-  const float* w = param(weight, x, "weight");
-  const float* b = param(bias, x, "bias");
+  const at::Tensor wt = param(weight, x, "weight"), bt = param(bias, x, "bias");
+  const float *w = pointer(wt), *b = pointer(bt);
   auto y = at::empty_like(x, x.options(), at::MemoryFormat::ChannelsLast);
   at::Tensor stats;
   if (keep_stats)
@@ -90,8 +94,8 @@ std::vector<at::Tensor> group_norm_backward(
               "group_norm: gy must be like x");
   c10::DeviceGuard guard(x.device());
   const DropoutArgs d = dropout_args(p, rng, seed, offset, x);
-  const float* w = param(weight, x, "weight");
-  const float* b = param(bias, x, "bias");
+  const at::Tensor wt = param(weight, x, "weight"), bt = param(bias, x, "bias");
+  const float *w = pointer(wt), *b = pointer(bt);
   at::Tensor dx, dw, db;
   const auto opts = x.options().dtype(at::kFloat);
   if (need_x) dx = at::empty_like(x, x.options(), at::MemoryFormat::ChannelsLast);

@@ -50,14 +50,19 @@ constexpr int THREADS = 512;      // of a block that sums
 constexpr int BLOCK = 256;        // of a block that does not
 using Shape = GroupNormShape;
 
-// Pixels cut into n pieces, the first `more` of them one longer than `size`.
-struct Cut {
-  int n, size, more;
-  __device__ __forceinline__ int first(int i) const {
-    return i * size + min(i, more);
-  }
+// A sample's pixels dealt to n blocks: batches of `batch` pixels, of which
+// block i takes i, i + n, ...  Blocks that run together then read neighbouring
+// memory.  (Each with a long piece of its own, whose lengths are large powers
+// of 2 here, they met at the same memory channels: 403 MB took 113 us to read,
+// not 70.)
+struct Deal {
+  int n, batch, batches, missing;  // missing: pixels that the last batch lacks
   __device__ __forceinline__ int pixels(int i) const {
-    return size + (i < more ? 1 : 0);
+    const int k = (batches - i + n - 1) / n;
+    return k * batch - ((batches - 1) % n == i ? missing : 0);
+  }
+  __device__ __forceinline__ int length(int k) const {  // of batch k
+    return batch - (k == batches - 1 ? missing : 0);
   }
 };
 
@@ -83,10 +88,16 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+// a / b for 0 <= a < 2^20, b > 0, by a reciprocal: (a + 1/2) / b is at least
+// 1 / (2 b) from the next integer, and off by less.
+__device__ __forceinline__ int small_div(int a, int b) {
+  return (int)(((float)a + 0.5f) * __builtin_amdgcn_rcpf((float)b));
+}
+
 // f(j, group of channel ch + j) for j < V, with one division.
 template <int V, typename F>
 __device__ __forceinline__ void each_group(int ch, int cg, F f) {
-  int g = ch / cg, r = ch - g * cg;
+  int g = small_div(ch, cg), r = ch - g * cg;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     f(j, g);
@@ -107,8 +118,8 @@ struct Place {
   int cols, rows, row, col;
   bool on;
   __device__ __forceinline__ Place(int cols_, int threads) : cols(cols_) {
-    rows = threads / cols;
-    row = threadIdx.x / cols;
+    rows = small_div(threads, cols);
+    row = small_div(threadIdx.x, cols);
     col = threadIdx.x - row * cols;
     on = row < rows;
   }
@@ -174,12 +185,13 @@ __device__ __forceinline__ void sum_groups(const F* red, const Place& pl,
                                            Done done) {
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
   const int last = first + width;
-  for (int g = first / upg + wave; g * upg < last; g += THREADS / WAVE) {
+  for (int g = small_div(first, upg) + wave; g * upg < last;
+       g += THREADS / WAVE) {
     const int lo = max(g * upg, first) - first;
     const int here = min((g + 1) * upg, last) - first - lo;
     // a lane's next entry is 64 further: so many rows and so many units
-    const int skip_r = WAVE / here, skip_u = WAVE - skip_r * here;
-    int r = lane / here, u = lane - r * here;
+    const int skip_r = small_div(WAVE, here), skip_u = WAVE - skip_r * here;
+    int r = small_div(lane, here), u = lane - r * here;
     F sum{};
     while (r < pl.rows) {
       add_to(sum, red[r * width + lo + u]);
@@ -219,9 +231,10 @@ struct Moments {
   }
   // (s1, s2) -> (mean, squares about it) of n values
   __device__ __forceinline__ void close(float n) {
+    const float inv = 1.0f / n;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float m = s1[j] / n;
+      const float m = s1[j] * inv;
       s2[j] = fmaxf(s2[j] - s1[j] * m, 0.0f);
       s1[j] = k[j] + m;
     }
@@ -338,7 +351,8 @@ __device__ __forceinline__ void weigh_groups(const float* s1, const float* s2,
                                              Fold fold) {
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
   const int last = first + width;
-  for (int g = first / cg + wave; g * cg < last; g += THREADS / WAVE) {
+  for (int g = small_div(first, cg) + wave; g * cg < last;
+       g += THREADS / WAVE) {
     const int lo = max(g * cg, first), hi = min((g + 1) * cg, last);
     float a = 0.0f, c = 0.0f;
     for (int i = lo + lane; i < hi; i += WAVE) {
@@ -355,6 +369,13 @@ __device__ __forceinline__ void weigh_groups(const float* s1, const float* s2,
 // ---------------------------------------------------------------------------
 // values
 // ---------------------------------------------------------------------------
+template <int V>
+__device__ __forceinline__ void load_floats(float (&v)[V], const float* at) {
+  const Pack<float, V> p = load_pack<float, V>(at);
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = p.v[j];
+}
+
 // z = (x - m) a + o, per channel of a thread's vector: a = rstd w, o = b.
 // Parameters first: they can be on their way while statistics are not known.
 template <int V>
@@ -364,8 +385,23 @@ struct Affine {
                                          const float* __restrict__ bias) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      a[j] = w ? w[ch + j] : 1.0f;
-      o[j] = bias ? bias[ch + j] : 0.0f;
+      a[j] = 1.0f;
+      o[j] = 0.0f;
+    }
+    if (w) load_floats<V>(a, w + ch);
+    if (bias) load_floats<V>(o, bias + ch);
+  }
+  // from [2][b][c] of mean and rstd w
+  __device__ __forceinline__ void channels(const float* chan, int64_t plane,
+                                           const float* __restrict__ bias,
+                                           int ch) {
+    load_floats<V>(m, chan);
+    load_floats<V>(a, chan + plane);
+    if (bias) {
+      load_floats<V>(o, bias + ch);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[j] = 0.0f;
     }
   }
   // indexed by group; channel ch is the thread's first
@@ -407,8 +443,42 @@ __device__ __forceinline__ void through(const Affine<V>& k,
     e[j] -= k.m[j];
     z[j] = fmaf(e[j], k.a[j], k.o[j]);
   }
-  act_backward<ACT, V>(act, z, g);
+  act_backward<T, ACT, V>(act, z, g);
   if (DROP && d.on) dropout_apply<V>(d, st, at, g);
+}
+
+// Vectors that a thread asks for at once, of one tensor or of each of two.
+template <typename T>
+constexpr int AHEAD1 = sizeof(T) == 2 ? 4 : 2;
+template <typename T>
+constexpr int AHEAD2 = sizeof(T) == 2 ? 4 : 2;
+
+template <typename T, int V>
+struct Both {
+  Pack<T, V> x, g;
+};
+
+// use(i, load(i)) for i < count, D loads ahead of their uses.  Loads stand
+// under no branch, or each would be waited for before the next: load(i, false)
+// is asked for something harmless past the end.
+template <int D, typename Load, typename Use>
+__device__ __forceinline__ void walk(int count, Load load, Use use) {
+  int i = 0;
+  for (; i + D <= count; i += D) {
+    decltype(load(0, true)) raw[D];
+#pragma unroll
+    for (int q = 0; q < D; ++q) raw[q] = load(i + q, true);
+#pragma unroll
+    for (int q = 0; q < D; ++q) use(i + q, raw[q]);
+  }
+  if (i < count) {
+    decltype(load(0, true)) raw[D - 1 > 0 ? D - 1 : 1];
+#pragma unroll
+    for (int q = 0; q < D - 1; ++q) raw[q] = load(i + q, i + q < count);
+#pragma unroll
+    for (int q = 0; q < D - 1; ++q)
+      if (i + q < count) use(i + q, raw[q]);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -420,13 +490,6 @@ struct Tiles {
   int iters;        // vectors per thread
 };
 
-// Vectors that a thread asks for at once, of one tensor or of each of two.  All
-// are asked for without a branch (past the end, the last one again): a load
-// under a condition is waited for before the next.
-template <typename T>
-constexpr int AHEAD1 = sizeof(T) == 2 ? 4 : 2;
-template <typename T>
-constexpr int AHEAD2 = sizeof(T) == 2 ? 4 : 2;
 
 // LDS: the tile, red, then floats per group.
 template <typename T, int V, int ACT, bool DROP>
@@ -443,35 +506,24 @@ __global__ __launch_bounds__(THREADS, 4) void gn_tile(
   const int span = blockIdx.x % tiles.spans, b = blockIdx.x / tiles.spans;
   const Place pl(tiles.span / V, THREADS);
   const int ch = span * tiles.span + pl.col * V;  // the thread's first channel
-  const int64_t from = (int64_t)b * s.hw * s.c + ch;
+  const int64_t from = ((int64_t)b * s.hw + pl.row) * s.c + ch;
+  const int64_t next = (int64_t)pl.rows * s.c;
   const int count = pl.count((int)s.hw);
 
-  auto load = [&](int i) {
-    return load_pack<T, V>(x + from + (int64_t)(pl.row + i * pl.rows) * s.c);
-  };
   Moments<V> t;
   t.begin();
   Affine<V> k;
   if (count) {
-    constexpr int D = AHEAD1<T>;
-    for (int i = 0; i < count; i += D) {
-      Pack<T, V> raw[D];
-#pragma unroll
-      for (int q = 0; q < D; ++q) raw[q] = load(min(i + q, count - 1));
-      if (i == 0) k.params(ch, w, bias);
+    k.params(ch, w, bias);
+    walk<AHEAD1<T>>(count, [&](int i, bool in) {
+      return load_pack<T, V>(x + from + (in ? i * next : 0));
+    }, [&](int i, const Pack<T, V>& raw) {
+      slots[i * THREADS + threadIdx.x] = raw;
       float v[V];
-      if (i == 0) {
-        unpack<T, V>(raw[0], v);
-        t.about(v);
-      }
-#pragma unroll
-      for (int q = 0; q < D; ++q) {
-        if (i + q >= count) continue;
-        slots[(i + q) * THREADS + threadIdx.x] = raw[q];
-        unpack<T, V>(raw[q], v);
-        t.add(v);
-      }
-    }
+      unpack<T, V>(raw, v);
+      if (i == 0) t.about(v);
+      t.add(v);
+    });
   }
   const float n = (float)s.hw * (float)s.cg;
   join_moments<V>(t, count, red, mean, pl, 0, s.cg, units,
@@ -491,7 +543,7 @@ __global__ __launch_bounds__(THREADS, 4) void gn_tile(
   const DropoutState st = dropout_state(d);
   k.stats(pl.col * V, s.cg, mean, rstd);
   for (int i = 0; i < count; ++i) {
-    const int64_t at = from + (int64_t)(pl.row + i * pl.rows) * s.c;
+    const int64_t at = from + i * next;
     store_pack<T, V>(y + at,
                      forward_value<T, V, ACT, DROP>(
                          k, slots[i * THREADS + threadIdx.x], act, d, st,
@@ -519,7 +571,8 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_tile(
   const int span = blockIdx.x % tiles.spans, b = blockIdx.x / tiles.spans;
   const Place pl(tiles.span / V, THREADS);
   const int c0 = span * tiles.span, ch = c0 + pl.col * V;
-  const int64_t from = (int64_t)b * s.hw * s.c + ch;
+  const int64_t from = ((int64_t)b * s.hw + pl.row) * s.c + ch;
+  const int64_t next = (int64_t)pl.rows * s.c;
   const int count = pl.count((int)s.hw);
   const DropoutState st = dropout_state(d);
   mean += (int64_t)b * s.g;
@@ -529,36 +582,24 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_tile(
   float s1[V], s2[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0f;
-  auto place = [&](int i) {
-    return from + (int64_t)(pl.row + i * pl.rows) * s.c;
-  };
   if (count) {
-    constexpr int D = AHEAD2<T> / 2;
     k.params(ch, w, bias);
     k.stats(ch, s.cg, mean, rstd);
-    for (int i = 0; i < count; i += D) {
-      Pack<T, V> rx[D], rg[D];
+    walk<AHEAD2<T> / 2>(count, [&](int i, bool in) {
+      const int64_t at = from + (in ? i * next : 0);
+      return Both<T, V>{load_pack<T, V>(x + at), load_pack<T, V>(gy + at)};
+    }, [&](int i, const Both<T, V>& raw) {
+      slots[i * THREADS + threadIdx.x] = raw.x;
+      slots[slot_g + i * THREADS + threadIdx.x] = raw.g;
+      float e[V], g[V];
+      through<T, V, ACT, DROP>(k, raw.x, raw.g, act, d, st,
+                               (uint64_t)(from + i * next), e, g);
 #pragma unroll
-      for (int q = 0; q < D; ++q) {
-        const int64_t at = place(min(i + q, count - 1));
-        rx[q] = load_pack<T, V>(x + at);
-        rg[q] = load_pack<T, V>(gy + at);
+      for (int j = 0; j < V; ++j) {
+        s1[j] += g[j];
+        s2[j] = fmaf(g[j], e[j], s2[j]);
       }
-#pragma unroll
-      for (int q = 0; q < D; ++q) {
-        if (i + q >= count) continue;
-        slots[(i + q) * THREADS + threadIdx.x] = rx[q];
-        slots[slot_g + (i + q) * THREADS + threadIdx.x] = rg[q];
-        float e[V], g[V];
-        through<T, V, ACT, DROP>(k, rx[q], rg[q], act, d, st,
-                                 (uint64_t)place(i + q), e, g);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          s1[j] += g[j];
-          s2[j] = fmaf(g[j], e[j], s2[j]);
-        }
-      }
-    }
+    });
   }
   if (count)
     each_group<V>(ch, s.cg, [&](int j, int g) { s2[j] *= rstd[g]; });
@@ -584,7 +625,7 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_tile(
     m2[j] = t2[g];
   });
   for (int i = 0; i < count; ++i) {
-    const int64_t at = from + (int64_t)(pl.row + i * pl.rows) * s.c;
+    const int64_t at = from + i * next;
     float e[V], g[V];
     through<T, V, ACT, DROP>(k, slots[i * THREADS + threadIdx.x],
                        slots[slot_g + i * THREADS + threadIdx.x], act, d, st,
@@ -604,7 +645,7 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_tile(
 // and groups that reach over chunks are joined as they come.
 template <typename T, int V>
 __global__ __launch_bounds__(THREADS, 4) void gn_stats(
-    const T* __restrict__ x, float2* __restrict__ part, Shape s, Cut cut,
+    const T* __restrict__ x, float2* __restrict__ part, Shape s, Deal deal,
     int units) {
   constexpr int D = AHEAD1<T>;
   __shared__ float2 red[THREADS * V];
@@ -613,32 +654,28 @@ __global__ __launch_bounds__(THREADS, 4) void gn_stats(
   float* jn = mean + s.g;
   float* jm = jn + s.g;
   float* jq = jm + s.g;
-  const int split = blockIdx.x % cut.n, b = blockIdx.x / cut.n;
-  const int pixels = cut.pixels(split);
-  const T* base = x + ((int64_t)b * s.hw + cut.first(split)) * s.c;
+  const int split = blockIdx.x % deal.n, b = blockIdx.x / deal.n;
+  const int pixels = deal.pixels(split);
+  const T* base = x + (int64_t)b * s.hw * s.c;
   for (int c0 = 0; c0 < s.c; c0 += THREADS * V) {
     const Place pl(min(THREADS, (s.c - c0) / V), THREADS);
-    const int count = pl.count(pixels);
     const int64_t next = (int64_t)pl.rows * s.c;
-    const T* at = base + (int64_t)pl.row * s.c + c0 + pl.col * V;
+    int count = 0;
     Moments<V> t;
     t.begin();
-    for (int i = 0; i < count; i += D) {
-      Pack<T, V> raw[D];
-#pragma unroll
-      for (int q = 0; q < D; ++q)
-        raw[q] = load_pack<T, V>(at + min(i + q, count - 1) * next);
-      float v[V];
-      if (i == 0) {
-        unpack<T, V>(raw[0], v);
-        t.about(v);
-      }
-#pragma unroll
-      for (int q = 0; q < D; ++q) {
-        if (i + q >= count) continue;
-        unpack<T, V>(raw[q], v);
+    for (int k = split; k < deal.batches; k += deal.n) {
+      const int here = pl.count(deal.length(k));
+      const T* at = base + ((int64_t)k * deal.batch + pl.row) * s.c + c0 +
+                    pl.col * V;
+      walk<D>(here, [&](int i, bool in) {
+        return load_pack<T, V>(at + (in ? i * next : 0));
+      }, [&](int i, const Pack<T, V>& raw) {
+        float v[V];
+        unpack<T, V>(raw, v);
+        if (i == 0 && k == split) t.about(v);
         t.add(v);
-      }
+      });
+      count += here;
     }
     const int last = c0 + pl.cols * V;
     // values of group g in this chunk
@@ -661,7 +698,7 @@ __global__ __launch_bounds__(THREADS, 4) void gn_stats(
                     });
   }
   for (int g = threadIdx.x; g < s.g; g += THREADS)
-    part[((int64_t)b * s.g + g) * cut.n + split] = make_float2(jm[g], jq[g]);
+    part[((int64_t)b * s.g + g) * deal.n + split] = make_float2(jm[g], jq[g]);
 }
 
 // `lanes` neighbouring threads, a power of two and at most a wave, share a
@@ -697,30 +734,44 @@ struct Share {
 };
 
 // A block per sample: joins the splits' statistics, the mean first, about
-// split 0's, then squares about it.  stat: [2][b][g] mean and rstd.
+// split 0's, then squares about it.  stat: [2][b][g] mean and rstd, kept for the
+// way back, or null.  chan: [2][b][c], mean and rstd w of every channel, which
+// the next launch's threads load as vectors.
 __global__ __launch_bounds__(THREADS) void gn_join(
-    const float2* __restrict__ part, float* __restrict__ stat, Shape s,
-    Cut cut, float eps) {
+    const float2* __restrict__ part, const float* __restrict__ w,
+    float* __restrict__ stat, float* __restrict__ chan, Shape s, Deal deal,
+    float eps) {
+  extern __shared__ float sums[];  // [2][g]
   const int b = blockIdx.x;
   const Share sh(s.g);
   for (int g = sh.group; g < s.g; g += sh.step) {
-    const float2* e = part + ((int64_t)b * s.g + g) * cut.n;
+    const float2* e = part + ((int64_t)b * s.g + g) * deal.n;
     const float ref = e[0].x;
     float sm = 0.0f, sq = 0.0f;
-    sh.each(e, cut.n, [&](int i, float2 v) {
-      sm += (float)cut.pixels(i) * (v.x - ref);
+    sh.each(e, deal.n, [&](int i, float2 v) {
+      sm += (float)deal.pixels(i) * (v.x - ref);
     });
     const float mean = ref + sh.sum(sm) / (float)s.hw;
-    sh.each(e, cut.n, [&](int i, float2 v) {
+    sh.each(e, deal.n, [&](int i, float2 v) {
       const float d = v.x - mean;
-      sq += fmaf((float)cut.pixels(i) * (float)s.cg, d * d, v.y);
+      sq += fmaf((float)deal.pixels(i) * (float)s.cg, d * d, v.y);
     });
     sq = sh.sum(sq);
     if (sh.lane == 0) {
-      stat[(int64_t)b * s.g + g] = mean;
-      stat[((int64_t)s.b + b) * s.g + g] =
-          rstd_of(sq, (float)s.hw * (float)s.cg, eps);
+      const float r = rstd_of(sq, (float)s.hw * (float)s.cg, eps);
+      sums[g] = mean;
+      sums[s.g + g] = r;
+      if (stat) {
+        stat[(int64_t)b * s.g + g] = mean;
+        stat[((int64_t)s.b + b) * s.g + g] = r;
+      }
     }
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < s.c; c += THREADS) {
+    const int g = c / s.cg;
+    chan[(int64_t)b * s.c + c] = sums[g];
+    chan[((int64_t)s.b + b) * s.c + c] = sums[s.g + g] * (w ? w[c] : 1.0f);
   }
 }
 
@@ -734,8 +785,8 @@ struct Pieces {
 
 template <typename T, int V, int ACT, bool DROP>
 __global__ __launch_bounds__(BLOCK) void gn_apply(
-    const T* __restrict__ x, T* __restrict__ y, const float* __restrict__ w,
-    const float* __restrict__ bias, const float* __restrict__ stat, Shape s,
+    const T* __restrict__ x, T* __restrict__ y,
+    const float* __restrict__ chan, const float* __restrict__ bias, Shape s,
     Pieces ps, bool stream, int act, DropoutArgs d) {
   const int chunk = blockIdx.x % ps.chunks, rest = blockIdx.x / ps.chunks;
   const int piece = rest % ps.pieces, b = rest / ps.pieces;
@@ -750,23 +801,15 @@ __global__ __launch_bounds__(BLOCK) void gn_apply(
   const DropoutState st = dropout_state(d);
   constexpr int D = AHEAD1<T>;
   Affine<V> k;
-  k.params(ch, w, bias);
-  k.stats(ch, s.cg, stat + (int64_t)b * s.g, stat + ((int64_t)s.b + b) * s.g);
-  for (int i = 0; i < count; i += D) {
-    Pack<T, V> raw[D];
-#pragma unroll
-    for (int q = 0; q < D; ++q)
-      raw[q] = load_pack<T, V>(x + from + min(i + q, count - 1) * next, stream);
-#pragma unroll
-    for (int q = 0; q < D; ++q) {
-      if (i + q >= count) continue;
-      const int64_t at = from + (i + q) * next;
-      store_pack<T, V>(y + at,
-                       forward_value<T, V, ACT, DROP>(k, raw[q], act, d, st,
-                                                      (uint64_t)at),
-                       stream);
-    }
-  }
+  k.channels(chan + (int64_t)b * s.c + ch, (int64_t)s.b * s.c, bias, ch);
+  walk<D>(count, [&](int i, bool in) {
+    return load_pack<T, V>(x + from + (in ? i * next : 0), stream);
+  }, [&](int i, const Pack<T, V>& raw) {
+    const int64_t at = from + i * next;
+    store_pack<T, V>(
+        y + at, forward_value<T, V, ACT, DROP>(k, raw, act, d, st, (uint64_t)at),
+        stream);
+  });
 }
 
 // Block (split, sample): sums of gz and gz xhat of every channel over the
@@ -777,58 +820,50 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_sums(
     const T* __restrict__ x, const T* __restrict__ gy,
     const float* __restrict__ w, const float* __restrict__ bias,
     const float* __restrict__ stat, float* __restrict__ part_c,
-    float2* __restrict__ part_g, Shape s, Cut cut, int act, DropoutArgs d) {
+    float2* __restrict__ part_g, Shape s, Deal deal, int act, DropoutArgs d) {
   extern __shared__ float lds_sums[];  // red; [2][channels]; [2][g]
   float* red = lds_sums;
   float* sum1 = red + RED_CHANNELS(V);
   float* sum2 = sum1 + min(THREADS * V, s.c);
   float* joined = sum2 + min(THREADS * V, s.c);
-  const int split = blockIdx.x % cut.n, b = blockIdx.x / cut.n;
+  const int split = blockIdx.x % deal.n, b = blockIdx.x / deal.n;
   const DropoutState st = dropout_state(d);
-  const int pixels = cut.pixels(split);
-  const int64_t from = ((int64_t)b * s.hw + cut.first(split)) * s.c;
   const float* mean = stat + (int64_t)b * s.g;
   const float* rstd = stat + ((int64_t)s.b + b) * s.g;
-  float* out1 = part_c + ((int64_t)b * cut.n + split) * s.c;
-  float* out2 = out1 + (int64_t)s.b * cut.n * s.c;
+  float* out1 = part_c + ((int64_t)b * deal.n + split) * s.c;
+  float* out2 = out1 + (int64_t)s.b * deal.n * s.c;
   for (int c0 = 0; c0 < s.c; c0 += THREADS * V) {
     const Place pl(min(THREADS, (s.c - c0) / V), THREADS);
-    const int count = pl.count(pixels);
     const int64_t next = (int64_t)pl.rows * s.c;
     const int ch = c0 + pl.col * V;
-    const int64_t at = from + (int64_t)pl.row * s.c + ch;
     float s1[V], s2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0f;
-    if (count) {
-      constexpr int D = AHEAD2<T>;
+    if (pl.on) {
+      constexpr int D = AHEAD2<T> / 2;  // more would spill registers
       Affine<V> k;
       k.params(ch, w, bias);
       k.stats(ch, s.cg, mean, rstd);
-      for (int i = 0; i < count; i += D) {
-        Pack<T, V> rx[D], rg[D];
-#pragma unroll
-        for (int q = 0; q < D; ++q) {
-          const int64_t to = at + min(i + q, count - 1) * next;
-          rx[q] = load_pack<T, V>(x + to);
-          rg[q] = load_pack<T, V>(gy + to);
-        }
-#pragma unroll
-        for (int q = 0; q < D; ++q) {
-          if (i + q >= count) continue;
+      for (int kb = split; kb < deal.batches; kb += deal.n) {
+        const int here = pl.count(deal.length(kb));
+        const int64_t at = ((int64_t)b * s.hw + (int64_t)kb * deal.batch +
+                            pl.row) * s.c + ch;
+        walk<D>(here, [&](int i, bool in) {
+          const int64_t to = at + (in ? i * next : 0);
+          return Both<T, V>{load_pack<T, V>(x + to), load_pack<T, V>(gy + to)};
+        }, [&](int i, const Both<T, V>& raw) {
           float e[V], g[V];
-          through<T, V, ACT, DROP>(k, rx[q], rg[q], act, d, st,
-                                   (uint64_t)(at + (i + q) * next), e, g);
+          through<T, V, ACT, DROP>(k, raw.x, raw.g, act, d, st,
+                                   (uint64_t)(at + i * next), e, g);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
             s1[j] += g[j];
             s2[j] = fmaf(g[j], e[j], s2[j]);
           }
-        }
+        });
       }
-    }
-    if (count)
       each_group<V>(ch, s.cg, [&](int j, int g) { s2[j] *= rstd[g]; });
+    }
     sum_channels<V>(red, pl, s1, s2, sum1, sum2);
     const int width = pl.cols * V;
     for (int c = threadIdx.x; c < width; c += THREADS) {
@@ -843,21 +878,25 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_sums(
     __syncthreads();
   }
   for (int g = threadIdx.x; g < s.g; g += THREADS)
-    part_g[((int64_t)b * s.g + g) * cut.n + split] =
+    part_g[((int64_t)b * s.g + g) * deal.n + split] =
         make_float2(joined[g], joined[s.g + g]);
 }
 
-// A block per sample: coef, [2][b][g], gets what dx adds to rstd w gz:
-// coef0 + (x - mean) coef1.
+// A block per sample.  chan: [4][b][c], for every channel its mean, rstd w, and
+// what dx adds to rstd w gz: chan2 + (x - mean) chan3.
 __global__ __launch_bounds__(THREADS) void gn_bwd_join(
-    const float2* __restrict__ part_g, const float* __restrict__ stat,
-    float* __restrict__ coef, Shape s, Cut cut) {
+    const float2* __restrict__ part_g, const float* __restrict__ w,
+    const float* __restrict__ stat, float* __restrict__ chan, Shape s,
+    Deal deal) {
+  extern __shared__ float sums[];  // [2][g]
   const int b = blockIdx.x;
   const Share sh(s.g);
   const float inv_n = 1.0f / ((float)s.hw * (float)s.cg);
+  const float* mean = stat + (int64_t)b * s.g;
+  const float* rstd = stat + ((int64_t)s.b + b) * s.g;
   for (int g = sh.group; g < s.g; g += sh.step) {
     float a = 0.0f, c = 0.0f;
-    sh.each(part_g + ((int64_t)b * s.g + g) * cut.n, cut.n,
+    sh.each(part_g + ((int64_t)b * s.g + g) * deal.n, deal.n,
             [&](int, float2 v) {
               a += v.x;
               c += v.y;
@@ -865,10 +904,19 @@ __global__ __launch_bounds__(THREADS) void gn_bwd_join(
     a = sh.sum(a);
     c = sh.sum(c);
     if (sh.lane == 0) {
-      const float r = stat[((int64_t)s.b + b) * s.g + g];
-      coef[(int64_t)b * s.g + g] = -r * (a * inv_n);
-      coef[((int64_t)s.b + b) * s.g + g] = -r * r * (c * inv_n);
+      sums[g] = -rstd[g] * (a * inv_n);
+      sums[s.g + g] = -rstd[g] * rstd[g] * (c * inv_n);
     }
+  }
+  __syncthreads();
+  const int64_t plane = (int64_t)s.b * s.c;
+  for (int c = threadIdx.x; c < s.c; c += THREADS) {
+    const int g = c / s.cg;
+    float* at = chan + (int64_t)b * s.c + c;
+    at[0] = mean[g];
+    at[plane] = rstd[g] * (w ? w[c] : 1.0f);
+    at[2 * plane] = sums[g];
+    at[3 * plane] = sums[s.g + g];
   }
 }
 
@@ -913,8 +961,7 @@ __global__ __launch_bounds__(BLOCK) void gn_param_grad(
 template <typename T, int V, int ACT, bool DROP>
 __global__ __launch_bounds__(BLOCK, 4) void gn_bwd_dx(
     const T* __restrict__ x, const T* __restrict__ gy, T* __restrict__ dx,
-    const float* __restrict__ w, const float* __restrict__ bias,
-    const float* __restrict__ stat, const float* __restrict__ coef,
+    const float* __restrict__ chan, const float* __restrict__ bias,
     const float* __restrict__ part_c, int64_t part_rows,
     float* __restrict__ db, float* __restrict__ dw, Shape s, Pieces ps,
     int param_blocks, bool stream, int act, DropoutArgs d) {
@@ -946,26 +993,18 @@ __global__ __launch_bounds__(BLOCK, 4) void gn_bwd_dx(
     store_pack<T, V>(dx + at, pack<T, V>(g), stream);
   };
   constexpr int D = AHEAD2<T>;
-  k.params(ch, w, bias);
-  k.stats(ch, s.cg, stat + (int64_t)b * s.g, stat + ((int64_t)s.b + b) * s.g);
-  const float* c0s = coef + (int64_t)b * s.g;
-  const float* c1s = c0s + (int64_t)s.b * s.g;
-  each_group<V>(ch, s.cg, [&](int j, int g) {
-    m1[j] = c0s[g];
-    m2[j] = c1s[g];
+  const int64_t plane = (int64_t)s.b * s.c;
+  chan += (int64_t)b * s.c + ch;
+  k.channels(chan, plane, bias, ch);
+  load_floats<V>(m1, chan + 2 * plane);
+  load_floats<V>(m2, chan + 3 * plane);
+  walk<D>(count, [&](int i, bool in) {
+    const int64_t at = from + (in ? i * next : 0);
+    return Both<T, V>{load_pack<T, V>(x + at, stream),
+                      load_pack<T, V>(gy + at, stream)};
+  }, [&](int i, const Both<T, V>& raw) {
+    emit(raw.x, raw.g, from + i * next);
   });
-  for (int i = 0; i < count; i += D) {
-    Pack<T, V> rx[D], rg[D];
-#pragma unroll
-    for (int q = 0; q < D; ++q) {
-      const int64_t at = from + min(i + q, count - 1) * next;
-      rx[q] = load_pack<T, V>(x + at, stream);
-      rg[q] = load_pack<T, V>(gy + at, stream);
-    }
-#pragma unroll
-    for (int q = 0; q < D; ++q)
-      if (i + q < count) emit(rx[q], rg[q], from + (i + q) * next);
-  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1029,14 +1068,16 @@ Plan plan_tiles(const Shape& s, int v, size_t value, bool back) {
   return p;
 }
 
-// Blocks per sample that sum: about 1024 over the batch, each with 16384
-// values or more; at most 256, which a join still reads at once.
-Cut cut_pixels(const Shape& s) {
-  int64_t n = (1024 + s.b - 1) / s.b;
-  n = std::min<int64_t>(n, s.hw * s.c / 16384);
-  n = std::max<int64_t>(1, std::min<int64_t>({n, s.hw, 256}));
-  TORCH_CHECK(s.b * n < (1ll << 31), "group_norm: tensor too large");
-  return {(int)n, (int)(s.hw / n), (int)(s.hw % n)};
+// Blocks per sample that sum: about 512 over the batch, two per CU, with `deep` vectors
+// per thread or more; at most 256, which a join still reads at once.
+Deal deal_pixels(const Shape& s, int v, int deep) {
+  Deal d;
+  d.batch = THREADS / std::min(THREADS, s.c / v) * deep;
+  d.batches = (int)((s.hw + d.batch - 1) / d.batch);
+  d.missing = (int)((int64_t)d.batches * d.batch - s.hw);
+  d.n = std::max(1, std::min({(512 + s.b - 1) / s.b, d.batches, 256}));
+  TORCH_CHECK((int64_t)s.b * d.n < (1ll << 31), "group_norm: tensor too large");
+  return d;
 }
 
 // Pieces of `deep` vectors per thread.
@@ -1116,28 +1157,31 @@ void gn_forward(const at::Tensor& x, at::Tensor& y, const float* w,
     });
     return;
   }
-  const Cut cut = cut_pixels(s);
-  const Pieces ps = cut_pieces(s, v, 8, 0);
-  auto buf = at::empty({(int64_t)s.b * s.g * (2 * cut.n + 2)},
+  const Deal deal = deal_pixels(s, v, AHEAD1<T>);
+  const Pieces ps = cut_pieces(s, v, 2 * AHEAD1<T>, 0);
+  const int64_t parts = (int64_t)s.b * s.g * deal.n;
+  const int64_t plane = (int64_t)s.b * s.c;
+  // channels' values first: their vectors are aligned
+  auto buf = at::empty({2 * plane + 2 * parts + 2},
                        x.options().dtype(at::kFloat));
-  float2* part = (float2*)buf.data_ptr();
-  if (!stat) stat = (float*)(part + (int64_t)s.b * s.g * cut.n);
+  float* chan = buf.data_ptr<float>();
+  float2* part = (float2*)(chan + 2 * plane);
   const auto stats = v == 8   ? gn_stats<T, 8>
                      : v == 4 ? gn_stats<T, 4>
                               : gn_stats<T, 1>;
   const size_t lds = 4 * (size_t)s.g * 4;
   allow_lds(stats, lds + THREADS * v * 8);
-  hipLaunchKernelGGL(stats, dim3(s.b * cut.n), dim3(THREADS), lds, stream, px,
-                     part, s, cut, p.units);
+  hipLaunchKernelGGL(stats, dim3(s.b * deal.n), dim3(THREADS), lds, stream, px,
+                     part, s, deal, p.units);
   C10_HIP_KERNEL_LAUNCH_CHECK();
-  hipLaunchKernelGGL(gn_join, dim3(s.b), dim3(THREADS), 0, stream, part, stat,
-                     s, cut, eps);
+  hipLaunchKernelGGL(gn_join, dim3(s.b), dim3(THREADS), 8 * s.g, stream, part,
+                     w, stat, chan, s, deal, eps);
   C10_HIP_KERNEL_LAUNCH_CHECK();
   const bool nt = x.numel() * (int64_t)sizeof(T) > STREAM_BYTES;
   GN_VARIANT(v, act, d.on, {
-    hipLaunchKernelGGL((gn_apply<T, V, ACT, DROP>), dim3(s.b * ps.pieces *
-                       ps.chunks), dim3(BLOCK), 0, stream, px, py, w, bias,
-                       stat, s, ps, nt, act, d);
+    hipLaunchKernelGGL((gn_apply<T, V, ACT, DROP>),
+                       dim3(s.b * ps.pieces * ps.chunks), dim3(BLOCK), 0,
+                       stream, px, py, chan, bias, s, ps, nt, act, d);
     C10_HIP_KERNEL_LAUNCH_CHECK();
   });
 }
@@ -1176,30 +1220,30 @@ void gn_backward(const at::Tensor& x, const at::Tensor& gy, at::Tensor& dx_out,
     }
     return;
   }
-  const Cut cut = cut_pixels(s);
-  const Pieces ps = cut_pieces(s, v, 4, param_blocks);
-  const int64_t rows = (int64_t)s.b * cut.n;
-  auto buf = at::empty({2 * rows * (s.c + s.g) + 2 * (int64_t)s.b * s.g}, opts);
-  float2* part_g = (float2*)buf.data_ptr();
-  float* part_c = (float*)(part_g + rows * s.g);
-  float* coef = part_c + 2 * rows * s.c;
+  const Deal deal = deal_pixels(s, v, AHEAD2<T>);
+  const Pieces ps = cut_pieces(s, v, 2 * AHEAD2<T>, param_blocks);
+  const int64_t rows = (int64_t)s.b * deal.n, plane = (int64_t)s.b * s.c;
+  auto buf = at::empty({4 * plane + 2 * rows * (s.c + s.g) + 2}, opts);
+  float* chan = buf.data_ptr<float>();
+  float* part_c = chan + 4 * plane;
+  float2* part_g = (float2*)(part_c + 2 * rows * s.c);
   const bool nt = x.numel() * (int64_t)sizeof(T) > STREAM_BYTES;
   GN_VARIANT(v, act, d.on, {
     auto sums = gn_bwd_sums<T, V, ACT, DROP>;
     const size_t lds =
         4 * (RED_CHANNELS(V) + 2 * (size_t)std::min(THREADS * V, s.c) + 2 * s.g);
     allow_lds(sums, lds);
-    hipLaunchKernelGGL(sums, dim3(s.b * cut.n), dim3(THREADS), lds, stream, px,
-                       pg, w, bias, stat, part_c, part_g, s, cut, act, d);
+    hipLaunchKernelGGL(sums, dim3(s.b * deal.n), dim3(THREADS), lds, stream, px,
+                       pg, w, bias, stat, part_c, part_g, s, deal, act, d);
     C10_HIP_KERNEL_LAUNCH_CHECK();
     if (dx) {
-      hipLaunchKernelGGL(gn_bwd_join, dim3(s.b), dim3(THREADS), 0, stream,
-                         part_g, stat, coef, s, cut);
+      hipLaunchKernelGGL(gn_bwd_join, dim3(s.b), dim3(THREADS), 8 * s.g, stream,
+                         part_g, w, stat, chan, s, deal);
       C10_HIP_KERNEL_LAUNCH_CHECK();
-      hipLaunchKernelGGL((gn_bwd_dx<T, V, ACT, DROP>), dim3(s.b * ps.pieces *
-                         ps.chunks + param_blocks), dim3(BLOCK), 0, stream, px,
-                         pg, dx, w, bias, stat, coef, part_c, rows, db, dw, s,
-                         ps, param_blocks, nt, act, d);
+      hipLaunchKernelGGL((gn_bwd_dx<T, V, ACT, DROP>),
+                         dim3(s.b * ps.pieces * ps.chunks + param_blocks),
+                         dim3(BLOCK), 0, stream, px, pg, dx, chan, bias, part_c,
+                         rows, db, dw, s, ps, param_blocks, nt, act, d);
     } else {
       hipLaunchKernelGGL(gn_param_grad, dim3(param_blocks), dim3(BLOCK), 0,
                          stream, part_c, rows, s.c, db, dw);

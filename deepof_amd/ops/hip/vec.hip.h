@@ -104,12 +104,20 @@ __device__ __forceinline__ float exp_f32(float z) {
              ? e : fmaf(e * 0.693147180559945f, r, e);
 }
 
+// The same for what ends in T.  In front of 16 bits, and of sums over many
+// values, t in one float will do: up to |z| = 16 it is 2^-20 off.
+template <typename T>
+__device__ __forceinline__ float exp_for(float z) {
+  if (sizeof(T) == 4) return exp_f32(z);
+  return __builtin_amdgcn_exp2f(z * 1.44269502162933349609375f);
+}
+
 // e^z - 1 for z <= 0.  Near 0 the subtraction would cancel: a Taylor sum
 // takes over where what it leaves out is below half a step of what is stored
 // (z^7 / 40320 < 2^-25 for fp32 results, z^3 / 24 < 2^-17 for 16 bits).
 template <typename T>
 __device__ __forceinline__ float expm1_neg(float z) {
-  const float far = exp_f32(z) - 1.0f;
+  const float far = exp_for<T>(z) - 1.0f;
   if (sizeof(T) == 4) {
     float s = 1.0f / 5040.0f;
     s = fmaf(s, z, 1.0f / 720.0f);
@@ -144,7 +152,7 @@ __device__ __forceinline__ void act_apply(int act, float (&v)[V]) {
     case ACT_SILU:
 #pragma unroll
       for (int k = 0; k < V; ++k)
-        v[k] = v[k] * __builtin_amdgcn_rcpf(1.0f + exp_f32(-v[k]));
+        v[k] = v[k] * __builtin_amdgcn_rcpf(1.0f + exp_for<T>(-v[k]));
       break;
     default:
       break;
@@ -152,13 +160,13 @@ __device__ __forceinline__ void act_apply(int act, float (&v)[V]) {
 }
 
 // g *= act'(z)
-template <int ACT, int V>
+template <typename T, int ACT, int V>
 __device__ __forceinline__ void act_backward(int act, const float (&z)[V],
                                              float (&g)[V]) {
   switch (ACT == ACT_ANY ? act : ACT) {
     case ACT_ELU:
 #pragma unroll
-      for (int k = 0; k < V; ++k) g[k] = z[k] <= 0.0f ? g[k] * exp_f32(z[k]) : g[k];
+      for (int k = 0; k < V; ++k) g[k] *= exp_for<T>(fminf(z[k], 0.0f));
       break;
     case ACT_LEAKY:
 #pragma unroll
@@ -171,7 +179,7 @@ __device__ __forceinline__ void act_backward(int act, const float (&z)[V],
     case ACT_SILU:
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const float t = __builtin_amdgcn_rcpf(1.0f + exp_f32(-z[k]));
+        const float t = __builtin_amdgcn_rcpf(1.0f + exp_for<T>(-z[k]));
         g[k] *= t * fmaf(z[k], 1.0f - t, 1.0f);
       }
       break;

@@ -189,6 +189,15 @@ def test_group_norm_without_parameters(have):
         assert_near(g, t, FP32, max(mx, mw, mb))
 
 
+def test_group_norm_parameters_at_any_address():
+    x = features((2, 16, 12, 10), BF16, 1)
+    w, b = params(16, 1)
+    want = oracle(x, 4, w, b, None)
+    both = torch.cat([torch.zeros(1), w, torch.zeros(2), b]).to(DEV)
+    got = ops.group_norm(x.to(DEV), 4, both[1:17], both[19:35])
+    assert_near(got, want, BF16, magnitudes(x, 4, w, b, None, 1.0))
+
+
 @pytest.mark.parametrize("which", [0, 1, 2])
 def test_group_norm_one_gradient_alone(which):
     x = features((3, 32, 20, 30), FP32, 5)
