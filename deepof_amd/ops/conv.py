@@ -233,6 +233,9 @@ class FusedConvAct(nn.Module):
                 times[name] = timeit(fn)
             except Exception:
                 pass
+        # autocast keeps the casts of weights made here, under no_grad, for
+        # the rest of its region: this step's weights would get no gradient
+        torch.clear_autocast_cache()
         choice = min(times, key=times.get)
         _dispatch_cache[key] = choice
         return choice

@@ -260,6 +260,8 @@ class FusedDeconvAct(torch.nn.Module):
             choice = "hip" if t_h < t_m else "miopen"
         except Exception:
             choice = "miopen"
+        # no gradient-free casts of weights stay behind (see FusedConvAct)
+        torch.clear_autocast_cache()
         _deconv_cache[key] = choice
         return choice
 
