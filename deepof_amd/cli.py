@@ -67,9 +67,10 @@ def main(argv=None):
         from .engine.evaluator import evaluate_aee
         from .engine.trainer import build_datasets
         from .losses.unsup import DATASET_MEANS
-        from .models import build_model
+        from .models import build_model, norm_kwargs
 
-        model, flow_scales, _ = build_model(cfg.model, act=cfg.activation)
+        model, flow_scales, _ = build_model(cfg.model, act=cfg.activation,
+                                            **norm_kwargs(cfg))
         device = torch.device("cuda" if cfg.device == "cuda"
                               and torch.cuda.is_available() else "cpu")
         model.to(device)
@@ -95,10 +96,11 @@ def main(argv=None):
         from .data.image import load_image, to_chw
         from .engine.evaluator import predict_flow
         from .losses.unsup import DATASET_MEANS
-        from .models import build_model
+        from .models import build_model, norm_kwargs
         from .utils import flow_to_color, write_flo
 
-        model, flow_scales, _ = build_model(cfg.model, act=cfg.activation)
+        model, flow_scales, _ = build_model(cfg.model, act=cfg.activation,
+                                            **norm_kwargs(cfg))
         device = torch.device("cuda" if cfg.device == "cuda"
                               and torch.cuda.is_available() else "cpu")
         model.to(device).eval()

@@ -34,6 +34,9 @@ class Config:
     # model
     model: str = "flownets"              # flownets|flownetc|vgg16|inception_v3
     activation: str = "elu"
+    norm: Optional[str] = None           # group; None = the model's own
+    feature_dropout: float = 0.0         # behind the features' activations
+    dropout_rng: str = "torch"           # classifier dropout: torch|counter
 
     augment: bool = False                # GPU geo+photo augmentation
     vgg_init: str = ""                   # path to vgg16_weights.npz warm start
@@ -94,6 +97,15 @@ class Config:
                 "augment=True with guided=True is unsupported: the GT "
                 "flow is not transformed through the geometric "
                 "augmentation (disable one of them)")
+
+        if self.norm not in (None, "group"):
+            raise ValueError(f"norm must be None or 'group', got {self.norm!r}")
+        if not 0.0 <= self.feature_dropout <= 1.0:
+            raise ValueError("feature_dropout must lie in [0, 1], got "
+                             f"{self.feature_dropout}")
+        if self.dropout_rng not in ("torch", "counter"):
+            raise ValueError("dropout_rng must be 'torch' or 'counter', got "
+                             f"{self.dropout_rng!r}")
 
     def to_dict(self):
         return dataclasses.asdict(self)

@@ -22,7 +22,7 @@ from ..data import (FlyingChairsDataset, SintelDataset, SyntheticFlowDataset,
                     UCF101Dataset, build_dataloader)
 from ..losses import MultiScaleGuidedLoss, MultiScaleUnsupLoss
 from ..losses.unsup import DATASET_MEANS
-from ..models import build_model
+from ..models import build_model, norm_kwargs
 from ..parallel import BucketedDataParallel, init_distributed
 from .evaluator import evaluate_aee
 from .optim import FusedAdam
@@ -59,7 +59,7 @@ class Trainer:
         )
         torch.manual_seed(cfg.seed + self.rank)
 
-        model_kwargs = {"act": cfg.activation}
+        model_kwargs = {"act": cfg.activation, **norm_kwargs(cfg)}
         if cfg.model == "inception_v3" and cfg.time_step > 2:
             model_kwargs["time_step"] = cfg.time_step
         if cfg.model in ("st_single", "st_baseline"):

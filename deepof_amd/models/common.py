@@ -27,14 +27,49 @@ def make_act(name: str) -> nn.Module:
     raise ValueError(f"unknown activation {name!r}")
 
 
+def check_norm(norm: str | None) -> None:
+    if norm not in (None, "group"):
+        raise ValueError(f"unknown norm {norm!r}; have None and 'group'")
+
+
+def _with_norm(build, cout: int, act: str | None, norm: str | None,
+               dropout: float) -> nn.Module:
+    """build(act) with a group norm between it and its activation, and dropout
+    behind that."""
+    from ..ops.norm import CounterDropout, GroupNormAct
+
+    check_norm(norm)
+    if norm == "group":
+        return nn.Sequential(build(None), GroupNormAct(cout, act,
+                                                       dropout=dropout))
+    if dropout:
+        return nn.Sequential(build(None), CounterDropout(dropout, act))
+    return build(act)
+
+
+def act_dropout(act: str, p: float, rng: str) -> list[nn.Module]:
+    """Activation and dropout of a classifier's hidden layer: torch's modules,
+    or ("counter") the fused operator in the second one's place."""
+    from ..ops.norm import CounterDropout
+
+    if rng == "torch":
+        return [make_act(act), nn.Dropout(p)]
+    if rng == "counter":
+        return [nn.Identity(), CounterDropout(p, act)]
+    raise ValueError(f"unknown dropout_rng {rng!r}; have 'torch' and 'counter'")
+
+
 def conv(cin: int, cout: int, k: int = 3, stride: int = 1,
-         act: str | None = "elu") -> nn.Module:
+         act: str | None = "elu", norm: str | None = None,
+         dropout: float = 0.0) -> nn.Module:
     from ..ops.conv import FusedConvAct
 
-    return FusedConvAct(cin, cout, k, stride, act)
+    return _with_norm(lambda a: FusedConvAct(cin, cout, k, stride, a), cout,
+                      act, norm, dropout)
 
 
-def deconv(cin: int, cout: int, act: str | None = "elu") -> nn.Module:
+def deconv(cin: int, cout: int, act: str | None = "elu",
+           norm: str | None = None, dropout: float = 0.0) -> nn.Module:
     """4x4 stride-2 transposed conv: exact 2x upsample (out = 2*in).
 
     On GPU the sub-pixel MFMA kernel runs it as 4 parity stride-1 convs
@@ -42,7 +77,8 @@ def deconv(cin: int, cout: int, act: str | None = "elu") -> nn.Module:
     nn.ConvTranspose2d."""
     from ..ops.deconv import FusedDeconvAct
 
-    return FusedDeconvAct(cin, cout, act)
+    return _with_norm(lambda a: FusedDeconvAct(cin, cout, a), cout, act, norm,
+                      dropout)
 
 
 def bilinear_deconv_weight(cin: int, cout: int, k: int = 4) -> torch.Tensor:
@@ -95,6 +131,8 @@ class FlowDecoder(nn.Module):
             [512, 256, 128, 64, 32].
         flow_channels: 2 for a single pair, 2*(T-1) for multi-frame
             Sintel volumes (sintelWrapFlow.py:386).
+        norm, dropout: None or "group", and a probability, for the upsampled
+            features (`conv`); flow heads have neither.
 
     forward(features) -> list of raw flow predictions, COARSEST first
     ([pr6 ... pr1] in reference naming).
@@ -102,7 +140,8 @@ class FlowDecoder(nn.Module):
 
     def __init__(self, feat_channels: list[int], up_channels: list[int],
                  act: str = "elu", flow_channels: int = 2,
-                 up_factors: list[int] | None = None):
+                 up_factors: list[int] | None = None,
+                 norm: str | None = None, dropout: float = 0.0):
         super().__init__()
         assert len(up_channels) == len(feat_channels) - 1
         self.num_scales = len(feat_channels)
@@ -113,11 +152,12 @@ class FlowDecoder(nn.Module):
         self.upconvs = nn.ModuleList()
         self.upflows = nn.ModuleList()
 
-        def up(cin, cout, factor, a):
+        def up(cin, cout, factor, a, **kw):
             # factor 1 happens between two same-resolution skips
             # (Inception's MaxPool_5a / Mixed_5d pair,
             # sintelWrapFlow.py:413-417 with scale=1)
-            return deconv(cin, cout, act=a) if factor == 2 else conv(cin, cout, 3, 1, a)
+            return (deconv(cin, cout, act=a, **kw) if factor == 2
+                    else conv(cin, cout, 3, 1, a, **kw))
 
         # concat channels padded to 64-multiples so the decoder's convs,
         # flow heads and upconvs are MFMA-kernel-eligible (1026/770/386/
@@ -127,7 +167,8 @@ class FlowDecoder(nn.Module):
         for i in range(self.num_scales):
             self.flow_heads.append(conv(concat_ch, flow_channels, 3, act=None))
             if i < self.num_scales - 1:
-                self.upconvs.append(up(concat_ch, up_channels[i], up_factors[i], act))
+                self.upconvs.append(up(concat_ch, up_channels[i], up_factors[i], act,
+                                       norm=norm, dropout=dropout))
                 uf = up(flow_channels, flow_channels, up_factors[i], None)
                 from ..ops.deconv import FusedDeconvAct
 

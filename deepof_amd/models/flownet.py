@@ -28,21 +28,23 @@ class FlowNetS(nn.Module):
     num_scales = 6
     # finest -> coarsest, matching FLOW_SCALES order after reversal
     def __init__(self, act: str = "elu", in_channels: int = 6,
-                 flow_channels: int = 2):
+                 flow_channels: int = 2, norm: str | None = None,
+                 feature_dropout: float = 0.0):
         super().__init__()
-        self.conv1 = conv(in_channels, 64, 7, 2, act)
-        self.conv2 = conv(64, 128, 5, 2, act)
-        self.conv3_1 = conv(128, 256, 5, 2, act)
-        self.conv3_2 = conv(256, 256, 3, 1, act)
-        self.conv4_1 = conv(256, 512, 3, 2, act)
-        self.conv4_2 = conv(512, 512, 3, 1, act)
-        self.conv5_1 = conv(512, 512, 3, 2, act)
-        self.conv5_2 = conv(512, 512, 3, 1, act)
-        self.conv6_1 = conv(512, 1024, 3, 2, act)
-        self.conv6_2 = conv(1024, 1024, 3, 1, act)
+        extra = {"norm": norm, "dropout": feature_dropout}
+        self.conv1 = conv(in_channels, 64, 7, 2, act, **extra)
+        self.conv2 = conv(64, 128, 5, 2, act, **extra)
+        self.conv3_1 = conv(128, 256, 5, 2, act, **extra)
+        self.conv3_2 = conv(256, 256, 3, 1, act, **extra)
+        self.conv4_1 = conv(256, 512, 3, 2, act, **extra)
+        self.conv4_2 = conv(512, 512, 3, 1, act, **extra)
+        self.conv5_1 = conv(512, 512, 3, 2, act, **extra)
+        self.conv5_2 = conv(512, 512, 3, 1, act, **extra)
+        self.conv6_1 = conv(512, 1024, 3, 2, act, **extra)
+        self.conv6_2 = conv(1024, 1024, 3, 1, act, **extra)
         self.decoder = FlowDecoder(
             [1024, 512, 512, 256, 128, 64], [512, 256, 128, 64, 32],
-            act=act, flow_channels=flow_channels,
+            act=act, flow_channels=flow_channels, **extra,
         )
         init_flow_module(self)
 
@@ -68,23 +70,26 @@ class FlowNetS(nn.Module):
 class FlowNetC(nn.Module):
     num_scales = 6
 
-    def __init__(self, act: str = "elu", max_displacement: int = 10):
+    def __init__(self, act: str = "elu", max_displacement: int = 10,
+                 norm: str | None = None, feature_dropout: float = 0.0):
         super().__init__()
+        extra = {"norm": norm, "dropout": feature_dropout}
         self.md = max_displacement
-        self.conv1 = conv(3, 64, 7, 2, act)
-        self.conv2 = conv(64, 128, 5, 2, act)
-        self.conv3 = conv(128, 256, 5, 2, act)
-        self.conv_redir = conv(256, 32, 1, 1, act)
+        self.conv1 = conv(3, 64, 7, 2, act, **extra)
+        self.conv2 = conv(64, 128, 5, 2, act, **extra)
+        self.conv3 = conv(128, 256, 5, 2, act, **extra)
+        self.conv_redir = conv(256, 32, 1, 1, act, **extra)
         corr_ch = (2 * max_displacement + 1) ** 2
-        self.conv3_1 = conv(corr_ch + 32, 256, 3, 1, act)
-        self.conv4_1 = conv(256, 512, 3, 2, act)
-        self.conv4_2 = conv(512, 512, 3, 1, act)
-        self.conv5_1 = conv(512, 512, 3, 2, act)
-        self.conv5_2 = conv(512, 512, 3, 1, act)
-        self.conv6_1 = conv(512, 1024, 3, 2, act)
-        self.conv6_2 = conv(1024, 1024, 3, 1, act)
+        self.conv3_1 = conv(corr_ch + 32, 256, 3, 1, act, **extra)
+        self.conv4_1 = conv(256, 512, 3, 2, act, **extra)
+        self.conv4_2 = conv(512, 512, 3, 1, act, **extra)
+        self.conv5_1 = conv(512, 512, 3, 2, act, **extra)
+        self.conv5_2 = conv(512, 512, 3, 1, act, **extra)
+        self.conv6_1 = conv(512, 1024, 3, 2, act, **extra)
+        self.conv6_2 = conv(1024, 1024, 3, 1, act, **extra)
         self.decoder = FlowDecoder(
-            [1024, 512, 512, 256, 128, 64], [512, 256, 128, 64, 32], act=act
+            [1024, 512, 512, 256, 128, 64], [512, 256, 128, 64, 32], act=act,
+            **extra,
         )
         init_flow_module(self)
 

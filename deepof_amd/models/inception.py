@@ -19,6 +19,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
+from ..ops import CounterDropout, GroupNormAct
 from .common import FlowDecoder, init_flow_module
 
 # finest (pr1 at 1/2) -> coarsest (pr6 at 1/32); two 1/8 scales
@@ -34,6 +35,12 @@ class BasicConv2d(nn.Module):
                               bias=False)
         self.bn = nn.BatchNorm2d(cout, eps=0.001)
         self.act = nn.ReLU(inplace=True)
+
+    def use_group_norm(self, dropout: float = 0.0):
+        """In place of batch norm and its activation."""
+        self.bn = GroupNormAct(self.conv.out_channels, "relu",
+                               eps=self.bn.eps, dropout=dropout)
+        self.act = nn.Identity()
 
     def forward(self, x):
         return self.act(self.bn(self.conv(x)))
@@ -178,7 +185,8 @@ class InceptionFlow(nn.Module):
     num_scales = 6
     flow_scales = INCEPTION_FLOW_SCALES
 
-    def __init__(self, act: str = "elu", time_step: int = 2):
+    def __init__(self, act: str = "elu", time_step: int = 2,
+                 norm: str | None = None, feature_dropout: float = 0.0):
         super().__init__()
         self.time_step = time_step
         flow_channels = 2 * (time_step - 1)
@@ -189,7 +197,17 @@ class InceptionFlow(nn.Module):
             act=act,
             flow_channels=flow_channels,
             up_factors=[2, 2, 1, 2, 2],
+            norm=norm,
+            dropout=feature_dropout,
         )
+        if norm == "group":
+            for m in self.encoder.modules():
+                if isinstance(m, BasicConv2d):
+                    m.use_group_norm(feature_dropout)
+        elif feature_dropout:
+            for m in self.encoder.modules():
+                if isinstance(m, BasicConv2d):
+                    m.act = CounterDropout(feature_dropout, "relu")
         init_flow_module(self)
 
     def forward(self, x: torch.Tensor) -> list[torch.Tensor]:

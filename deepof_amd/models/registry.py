@@ -46,6 +46,15 @@ MODEL_REGISTRY = {
 }
 
 
+def norm_kwargs(cfg) -> dict:
+    """What a config says of normalisation and dropout, as arguments of its
+    model; a model's parameters depend on the first of them."""
+    kwargs = {"norm": cfg.norm, "feature_dropout": cfg.feature_dropout}
+    if cfg.model in ("st_single", "st_baseline"):
+        kwargs["dropout_rng"] = cfg.dropout_rng
+    return kwargs
+
+
 def build_model(name: str, **kwargs):
     if name not in MODEL_REGISTRY:
         raise ValueError(f"unknown model {name!r}; have {sorted(MODEL_REGISTRY)}")

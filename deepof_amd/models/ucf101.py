@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
-from .common import FlowDecoder, conv, init_flow_module, make_act
+from .common import FlowDecoder, act_dropout, conv, init_flow_module
 from .flownet import FlowNetS
 from .vgg16 import VGG16Encoder, VGG_FLOW_SCALES
 
@@ -27,16 +27,22 @@ class STSingle(nn.Module):
 
     def __init__(self, input_hw: tuple[int, int] = (256, 320),
                  num_classes: int = 101, act: str = "elu",
-                 fc_dim: int = 4096, dropout: float = 0.5):
+                 fc_dim: int = 4096, dropout: float = 0.5,
+                 dropout_rng: str = "torch", norm: str | None = None,
+                 feature_dropout: float = 0.0):
         super().__init__()
-        self.encoder = VGG16Encoder(6, act="relu")
+        self.encoder = VGG16Encoder(6, act="relu", norm=norm,
+                                    feature_dropout=feature_dropout)
         self.decoder = FlowDecoder([512, 512, 256, 128, 64],
-                                   [256, 128, 64, 32], act=act)
+                                   [256, 128, 64, 32], act=act, norm=norm,
+                                   dropout=feature_dropout)
         h, w = input_hw
         flat_dim = (h // 32) * (w // 32) * 512
         self.classifier = nn.Sequential(
-            nn.Linear(flat_dim, fc_dim), make_act("relu"), nn.Dropout(dropout),
-            nn.Linear(fc_dim, fc_dim), make_act("relu"), nn.Dropout(dropout),
+            nn.Linear(flat_dim, fc_dim),
+            *act_dropout("relu", dropout, dropout_rng),
+            nn.Linear(fc_dim, fc_dim),
+            *act_dropout("relu", dropout, dropout_rng),
             nn.Linear(fc_dim, num_classes),
         )
         init_flow_module(self)
@@ -57,17 +63,22 @@ class STBaseline(nn.Module):
 
     def __init__(self, input_hw: tuple[int, int] = (256, 320),
                  num_classes: int = 101, act: str = "elu",
-                 fc_dim: int = 4096, dropout: float = 0.5):
+                 fc_dim: int = 4096, dropout: float = 0.5,
+                 dropout_rng: str = "torch", norm: str | None = None,
+                 feature_dropout: float = 0.0):
         super().__init__()
-        self.temporal = FlowNetS(act=act)
-        self.spatial = VGG16Encoder(3, act="relu")
+        extra = {"norm": norm, "feature_dropout": feature_dropout}
+        self.temporal = FlowNetS(act=act, **extra)
+        self.spatial = VGG16Encoder(3, act="relu", **extra)
         # fuse pool5 (512) with conv5_2 features (512) -> 512
-        self.fuse = conv(1024, 512, 1, 1, "relu")
+        self.fuse = conv(1024, 512, 1, 1, "relu", norm, feature_dropout)
         h, w = input_hw
         flat_dim = (h // 32) * (w // 32) * 512
         self.classifier = nn.Sequential(
-            nn.Linear(flat_dim, fc_dim), make_act("relu"), nn.Dropout(dropout),
-            nn.Linear(fc_dim, fc_dim), make_act("relu"), nn.Dropout(dropout),
+            nn.Linear(flat_dim, fc_dim),
+            *act_dropout("relu", dropout, dropout_rng),
+            nn.Linear(fc_dim, fc_dim),
+            *act_dropout("relu", dropout, dropout_rng),
             nn.Linear(fc_dim, num_classes),
         )
         init_flow_module(self.fuse)

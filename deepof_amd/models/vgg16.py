@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
-from .common import FlowDecoder, conv, init_flow_module, make_act
+from .common import FlowDecoder, act_dropout, conv, init_flow_module
 
 # flow scale at level k (pr1 at 1/2 resolution): 20 / 2^k
 VGG_FLOW_SCALES = [20.0 / (1 << k) for k in range(1, 6)]  # 5 scales
@@ -21,13 +21,16 @@ VGG_FLOW_SCALES = [20.0 / (1 << k) for k in range(1, 6)]  # 5 scales
 class VGG16Encoder(nn.Module):
     """conv1_1..conv5_3 with 2x2 max pools; returns the 5 pool outputs."""
 
-    def __init__(self, in_channels: int = 6, act: str = "relu"):
+    def __init__(self, in_channels: int = 6, act: str = "relu",
+                 norm: str | None = None, feature_dropout: float = 0.0):
         super().__init__()
+        extra = {"norm": norm, "dropout": feature_dropout}
 
         def block(cin, cout, n):
             layers = []
             for i in range(n):
-                layers.append(conv(cin if i == 0 else cout, cout, 3, 1, act))
+                layers.append(conv(cin if i == 0 else cout, cout, 3, 1, act,
+                                   **extra))
             return nn.Sequential(*layers)
 
         self.block1 = block(in_channels, 64, 2)
@@ -51,13 +54,16 @@ class VGG16Flow(nn.Module):
 
     num_scales = 5
 
-    def __init__(self, act: str = "elu", in_channels: int = 6):
+    def __init__(self, act: str = "elu", in_channels: int = 6,
+                 norm: str | None = None, feature_dropout: float = 0.0):
         super().__init__()
         # The reference keeps ReLU inside the VGG stack and ELU for the
         # decoder (ucf101wrapFlow.py uses ReLU for the classifier path).
-        self.encoder = VGG16Encoder(in_channels, act="relu")
+        self.encoder = VGG16Encoder(in_channels, act="relu", norm=norm,
+                                    feature_dropout=feature_dropout)
         self.decoder = FlowDecoder([512, 512, 256, 128, 64],
-                                   [256, 128, 64, 32], act=act)
+                                   [256, 128, 64, 32], act=act, norm=norm,
+                                   dropout=feature_dropout)
         init_flow_module(self)
 
     def forward(self, x: torch.Tensor) -> list[torch.Tensor]:
@@ -71,16 +77,16 @@ class VGG16Classifier(nn.Module):
 
     def __init__(self, input_hw: tuple[int, int], num_classes: int = 101,
                  in_channels: int = 3, fc_dim: int = 4096,
-                 dropout: float = 0.5):
+                 dropout: float = 0.5, dropout_rng: str = "torch"):
         super().__init__()
         self.encoder = VGG16Encoder(in_channels, act="relu")
         h, w = input_hw
         flat_dim = (h // 32) * (w // 32) * 512
         self.head = nn.Sequential(
-            nn.Linear(flat_dim, fc_dim), make_act("relu"),
-            nn.Dropout(dropout),
-            nn.Linear(fc_dim, fc_dim), make_act("relu"),
-            nn.Dropout(dropout),
+            nn.Linear(flat_dim, fc_dim),
+            *act_dropout("relu", dropout, dropout_rng),
+            nn.Linear(fc_dim, fc_dim),
+            *act_dropout("relu", dropout, dropout_rng),
             nn.Linear(fc_dim, num_classes),
         )
 

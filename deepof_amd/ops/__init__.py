@@ -11,8 +11,11 @@ from .functional import (
     hip_available,
     require_hip,
 )
+from .norm import CounterDropout, GroupNormAct
 
 __all__ = [
+    "CounterDropout",
+    "GroupNormAct",
     "warp_bilinear",
     "resize_bilinear",
     "lrn",

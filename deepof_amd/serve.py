@@ -134,9 +134,10 @@ def serve_from_config(cfg, checkpoint: str | None, host: str, port: int):
     import uvicorn
 
     from .losses.unsup import DATASET_MEANS
-    from .models import build_model
+    from .models import build_model, norm_kwargs
 
-    model, flow_scales, _ = build_model(cfg.model, act=cfg.activation)
+    model, flow_scales, _ = build_model(cfg.model, act=cfg.activation,
+                                        **norm_kwargs(cfg))
     device = torch.device("cuda" if cfg.device == "cuda"
                           and torch.cuda.is_available() else "cpu")
     model.to(device)

@@ -649,3 +649,54 @@ def test_refuses_tensors_of_other_devices():
         ops.dropout(x.to(DEV), 0.5, torch.tensor([1, 2]))
     with pytest.raises(TypeError):
         ops.dropout(x.to(DEV).double(), 0.5)
+
+
+# ---------------------------------------------------------------------------
+# together, as models use them
+# ---------------------------------------------------------------------------
+def test_block_as_models_build_it():
+    """conv -> norm + act + dropout -> conv -> act + dropout: the GPU's kernels
+    against the plain forms in 64 bits, the same masks on both sides."""
+    import torch.nn.functional as F
+
+    g = torch.Generator().manual_seed(50)
+    x = features((2, 8, 14, 18), FP32, 51)
+    w1, w2 = (torch.randn(16, c, 3, 3, generator=g) * 0.1 for c in (8, 16))
+    gamma, beta = params(16, 52)
+    gy = features((2, 16, 14, 18), FP32, 53)
+
+    def block(x, w1, w2, gamma, beta, norm, drop):
+        y = F.conv2d(x, w1, padding=1)
+        y = norm(y, 4, gamma, beta, act="elu", dropout=0.2, rng=(1, 2))
+        y = F.conv2d(y, w2, padding=1).contiguous(memory_format=LAST)
+        return drop(y, 0.3, (3, 4), act="silu")
+
+    leaves = [t.double().requires_grad_(True)
+              for t in (x, w1, w2, gamma, beta)]
+    want = block(*leaves, ops.group_norm, ops.dropout)  # CPU, 64 bits
+    dwant = torch.autograd.grad(want, leaves, gy.double())
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, w1, w2, gamma, beta)]
+    got = block(*leaves, ops.group_norm, ops.dropout)
+    dgot = torch.autograd.grad(got, leaves, gy.to(DEV))
+    # chains of two convolutions (72 and 144 terms) and a norm: 2^12 steps of
+    # fp32 relative to the largest value bound them
+    for a, t in zip((got,) + dgot, (want.detach(),) + dwant):
+        bound = 2.0**12 * 2.0**-24 * float(t.abs().max())
+        assert float((a.detach().cpu().double() - t).abs().max()) < bound
+
+
+@pytest.mark.parametrize("name", ["flownets", "inception_v3"])
+def test_model_step_with_group_norm(name):
+    from deepof_amd.models import build_model
+
+    torch.manual_seed(0)
+    model, _, _ = build_model(name, norm="group", feature_dropout=0.1)
+    model.to(DEV).to(memory_format=LAST)
+    x = torch.randn(2, 6, 128, 128, device=DEV).contiguous(memory_format=LAST)
+    with torch.autocast("cuda", dtype=BF16):
+        flows = model(x)
+    sum(f.float().square().mean() for f in flows).backward()
+    for n, p in model.named_parameters():
+        assert p.grad is not None and torch.isfinite(p.grad).all(), n
+    norms = [m for m in model.modules() if isinstance(m, ops.GroupNormAct)]
+    assert all(float(m.weight.grad.abs().sum()) > 0 for m in norms)

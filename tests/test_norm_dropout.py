@@ -196,3 +196,118 @@ X = torch.zeros(2, 8, 3, 3)
 def test_refusals(error, call):
     with pytest.raises(error):
         call("cpu")
+
+
+# ---------------------------------------------------------------------------
+# modules, models and configs
+# ---------------------------------------------------------------------------
+def test_modules_train_and_eval():
+    torch.manual_seed(0)
+    x = torch.randn(2, 48, 5, 6)
+    m = ops.GroupNormAct(48, "elu", dropout=0.5)
+    assert m.groups == 16
+    m.eval()
+    want = F.elu(F.group_norm(x, 16, m.weight, m.bias))
+    torch.testing.assert_close(m(x), want)
+    m.train()
+    assert 0.4 < float((m(x) == 0).float().mean()) < 0.6
+    d = ops.CounterDropout(0.5, "relu")
+    assert 0.7 < float((d(x) == 0).float().mean()) < 0.8
+    assert not torch.equal(d(x), d(x))
+    d.eval()
+    assert torch.equal(d(x), F.relu(x))
+    for bad in (lambda: ops.GroupNormAct(10, groups=3),
+                lambda: ops.GroupNormAct(8, "gelu"),
+                lambda: ops.GroupNormAct(8, dropout=2.0),
+                lambda: ops.CounterDropout(-1.0),
+                lambda: ops.CounterDropout(0.5, "tanh")):
+        with pytest.raises(ValueError):
+            bad()
+
+
+@pytest.mark.parametrize("name", ["flownets", "flownetc", "vgg16",
+                                  "inception_v3"])
+def test_models_with_group_norm(name):
+    from deepof_amd.models import build_model
+
+    torch.manual_seed(0)
+    model, scales, _ = build_model(name, norm="group", feature_dropout=0.1)
+    norms = [m for m in model.modules() if isinstance(m, ops.GroupNormAct)]
+    assert norms and all(m.dropout == 0.1 for m in norms)
+    assert not any(isinstance(m, torch.nn.BatchNorm2d)
+                   for m in model.modules())
+    x = torch.randn(1, 6, 64, 64)
+    flows = model(x)
+    assert len(flows) == len(scales) and flows[0].shape == (1, 2, 32, 32)
+    sum(f.square().sum() for f in flows).backward()
+    for p in model.parameters():
+        assert p.grad is not None and torch.isfinite(p.grad).all()
+    model.eval()
+    with torch.no_grad():
+        a, b = model(x), model(x)
+    assert all(torch.equal(s, t) for s, t in zip(a, b))
+
+
+def test_models_are_as_before_without():
+    from deepof_amd.models import build_model
+    from deepof_amd.models.ucf101 import STSingle
+
+    for name in ("flownets", "inception_v3"):
+        model, _, _ = build_model(name)
+        assert not any(isinstance(m, (ops.GroupNormAct, ops.CounterDropout))
+                       for m in model.modules())
+    kw = {"input_hw": (64, 64), "fc_dim": 32, "num_classes": 5}
+    plain, counter = STSingle(**kw), STSingle(**kw, dropout_rng="counter")
+    assert sum(isinstance(m, torch.nn.Dropout) for m in plain.modules()) == 2
+    assert sum(isinstance(m, ops.CounterDropout)
+               for m in counter.modules()) == 2
+    # one's checkpoint is the other's
+    counter.load_state_dict(plain.state_dict())
+    x = torch.randn(2, 6, 64, 64)
+    plain.eval(), counter.eval()
+    torch.testing.assert_close(counter(x)[1], plain(x)[1])
+    counter.train()
+    counter(x)[1].sum().backward()
+    with pytest.raises(ValueError):
+        STSingle(**kw, dropout_rng="other")
+    with pytest.raises(ValueError):
+        build_model("flownets", norm="layer")
+
+
+def test_inception_feature_dropout_without_group_norm():
+    from deepof_amd.models import build_model
+
+    model, _, _ = build_model("inception_v3", feature_dropout=0.2)
+    drops = [m for m in model.modules() if isinstance(m, ops.CounterDropout)]
+    assert drops and any(isinstance(m, torch.nn.BatchNorm2d)
+                         for m in model.modules())
+    model.eval()
+    with torch.no_grad():
+        assert torch.isfinite(model(torch.randn(1, 6, 64, 64))[0]).all()
+
+
+def test_config_keys():
+    from deepof_amd.config import Config
+
+    cfg = Config().apply_overrides(["norm=group", "feature_dropout=0.1",
+                                    "dropout_rng=counter"])
+    assert (cfg.norm, cfg.feature_dropout, cfg.dropout_rng) == (
+        "group", 0.1, "counter")
+    assert Config().norm is None and Config().dropout_rng == "torch"
+    for bad in ("norm=batch", "feature_dropout=1.5", "dropout_rng=x"):
+        with pytest.raises(ValueError):
+            Config().apply_overrides([bad])
+
+
+def test_train_then_eval_from_the_command_line(tmp_path, capsys):
+    """A checkpoint of a normed model is evaluated by the same config."""
+    from deepof_amd.cli import main
+
+    common = ["dataset=synthetic", "image_size=[64, 64]", "batch_size=2",
+              "num_workers=0", "device=cpu", "norm=group",
+              "feature_dropout=0.1", f"log_dir={tmp_path}", "run_name=r"]
+    main(["train", "--max-steps", "1"] + common)
+    ckpt = tmp_path / "r" / "ckpt_last.pt"
+    assert ckpt.exists()
+    main(["eval", "--checkpoint", str(ckpt)] + common)
+    assert "AEE" in capsys.readouterr().out
