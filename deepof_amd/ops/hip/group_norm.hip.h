@@ -46,6 +46,7 @@
 namespace {
 
 constexpr int WAVE = 64;
+constexpr int XCDS = 8;           // blocks go to them in turn, each with an L2
 constexpr int THREADS = 512;      // of a block that sums
 constexpr int BLOCK = 256;        // of a block that does not
 using Shape = GroupNormShape;
@@ -484,6 +485,15 @@ __device__ __forceinline__ void walk(int count, Load load, Use use) {
 // ---------------------------------------------------------------------------
 // tile route
 // ---------------------------------------------------------------------------
+// Tiles narrower than a cache line share lines with their neighbours.  Block
+// i's tile is so chosen that neighbours go to the same XCD, whose L2 then
+// fetches a line once, and writes it back whole.  (8x24x32x512 bf16, spans of
+// 32 bytes: 12.0 us without, and see gn_tile with.)
+__device__ __forceinline__ int neighbours_together(int i, int n) {
+  const int each = n / XCDS;
+  return i < each * XCDS ? (i % XCDS) * each + i / XCDS : i;
+}
+
 struct Tiles {
   int span, spans;  // channels of a tile, tiles of a sample
   int groups;       // groups of a tile
@@ -503,7 +513,8 @@ __global__ __launch_bounds__(THREADS, 4) void gn_tile(
   float2* red = reinterpret_cast<float2*>(slots + tiles.iters * THREADS);
   float* mean = reinterpret_cast<float*>(red + THREADS * units);
   float* rstd = mean + tiles.groups;
-  const int span = blockIdx.x % tiles.spans, b = blockIdx.x / tiles.spans;
+  const int at_tile = neighbours_together(blockIdx.x, gridDim.x);
+  const int span = at_tile % tiles.spans, b = at_tile / tiles.spans;
   const Place pl(tiles.span / V, THREADS);
   const int ch = span * tiles.span + pl.col * V;  // the thread's first channel
   const int64_t from = ((int64_t)b * s.hw + pl.row) * s.c + ch;
@@ -568,7 +579,8 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_tile(
   float* sum2 = sum1 + tiles.span;
   float* t1 = sum2 + tiles.span;
   float* t2 = t1 + tiles.groups;
-  const int span = blockIdx.x % tiles.spans, b = blockIdx.x / tiles.spans;
+  const int at_tile = neighbours_together(blockIdx.x, gridDim.x);
+  const int span = at_tile % tiles.spans, b = at_tile / tiles.spans;
   const Place pl(tiles.span / V, THREADS);
   const int c0 = span * tiles.span, ch = c0 + pl.col * V;
   const int64_t from = ((int64_t)b * s.hw + pl.row) * s.c + ch;
@@ -701,66 +713,84 @@ __global__ __launch_bounds__(THREADS, 4) void gn_stats(
     part[((int64_t)b * s.g + g) * deal.n + split] = make_float2(jm[g], jq[g]);
 }
 
-// `lanes` neighbouring threads, a power of two and at most a wave, share a
-// group and take every lanes-th of its partial sums, MOST at a time.
-constexpr int MOST = 8;
+// A group's partial sums are joined by `lanes` neighbouring threads, a power of
+// two and at most a wave, with up to MOST of them each: all are asked for at
+// once, and kept for a second pass.
+constexpr int MOST = 4;
+constexpr int MOST_PARTS = MOST * WAVE;
 
 struct Share {
-  int lanes, lane, group, step;
-  __device__ __forceinline__ explicit Share(int groups) {
-    lanes = WAVE;
-    while (lanes > 1 && lanes * groups > THREADS) lanes >>= 1;
-    lane = threadIdx.x & (lanes - 1);
-    group = threadIdx.x / lanes;
-    step = THREADS / lanes;
-  }
-  __device__ __forceinline__ float sum(float v) const {
-    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, WAVE);
-    return v;
-  }
-  // f(i, entry) over this thread's entries below n
-  template <typename F>
-  __device__ __forceinline__ void each(const float2* e, int n, F f) const {
-    for (int i = lane; i < n; i += MOST * lanes) {
-      float2 v[MOST];
-#pragma unroll
-      for (int q = 0; q < MOST; ++q)
-        if (i + q * lanes < n) v[q] = e[i + q * lanes];
-#pragma unroll
-      for (int q = 0; q < MOST; ++q)
-        if (i + q * lanes < n) f(i + q * lanes, v[q]);
-    }
-  }
+  int lanes, lane, group;   // group: among this block's
+  int groups, blocks;       // of a block, of a sample
 };
 
-// A block per sample: joins the splits' statistics, the mean first, about
+__host__ __device__ __forceinline__ int share_lanes(int parts) {
+  int lanes = 1;
+  while (lanes * MOST < parts) lanes *= 2;
+  return lanes;
+}
+
+__device__ __forceinline__ Share share_of(int lanes, int groups) {
+  Share sh;
+  sh.lanes = lanes;
+  sh.lane = threadIdx.x & (lanes - 1);
+  sh.groups = THREADS / lanes;
+  sh.group = threadIdx.x / lanes;
+  sh.blocks = (groups + sh.groups - 1) / sh.groups;
+  return sh;
+}
+
+__device__ __forceinline__ float share_sum(const Share& sh, float v) {
+  for (int o = sh.lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, WAVE);
+  return v;
+}
+
+// This thread's parts of e[0 .. n); zeros past the end.
+__device__ __forceinline__ void share_load(const Share& sh, const float2* e,
+                                           int n, float2 (&v)[MOST]) {
+#pragma unroll
+  for (int q = 0; q < MOST; ++q) {
+    const int i = sh.lane + q * sh.lanes;
+    v[q] = i < n ? e[i] : make_float2(0.0f, 0.0f);
+  }
+}
+
+// Block (groups, sample): joins the splits' statistics, the mean first, about
 // split 0's, then squares about it.  stat: [2][b][g] mean and rstd, kept for the
 // way back, or null.  chan: [2][b][c], mean and rstd w of every channel, which
 // the next launch's threads load as vectors.
 __global__ __launch_bounds__(THREADS) void gn_join(
     const float2* __restrict__ part, const float* __restrict__ w,
     float* __restrict__ stat, float* __restrict__ chan, Shape s, Deal deal,
-    float eps) {
-  extern __shared__ float sums[];  // [2][g]
-  const int b = blockIdx.x;
-  const Share sh(s.g);
-  for (int g = sh.group; g < s.g; g += sh.step) {
+    int lanes, float eps) {
+  __shared__ float sums[2][THREADS];
+  const Share sh = share_of(lanes, s.g);
+  const int b = blockIdx.x / sh.blocks;
+  const int g0 = (blockIdx.x - b * sh.blocks) * sh.groups;
+  const int g = g0 + sh.group;
+  if (g < s.g) {
     const float2* e = part + ((int64_t)b * s.g + g) * deal.n;
+    float2 v[MOST];
+    share_load(sh, e, deal.n, v);
     const float ref = e[0].x;
-    float sm = 0.0f, sq = 0.0f;
-    sh.each(e, deal.n, [&](int i, float2 v) {
-      sm += (float)deal.pixels(i) * (v.x - ref);
-    });
-    const float mean = ref + sh.sum(sm) / (float)s.hw;
-    sh.each(e, deal.n, [&](int i, float2 v) {
-      const float d = v.x - mean;
-      sq += fmaf((float)deal.pixels(i) * (float)s.cg, d * d, v.y);
-    });
-    sq = sh.sum(sq);
+    float n[MOST], sm = 0.0f, sq = 0.0f;
+#pragma unroll
+    for (int q = 0; q < MOST; ++q) {
+      const int i = sh.lane + q * sh.lanes;
+      n[q] = i < deal.n ? (float)deal.pixels(i) : 0.0f;
+      sm += n[q] * (v[q].x - ref);
+    }
+    const float mean = ref + share_sum(sh, sm) / (float)s.hw;
+#pragma unroll
+    for (int q = 0; q < MOST; ++q) {
+      const float d = v[q].x - mean;
+      sq += fmaf(n[q] * (float)s.cg, d * d, v[q].y);
+    }
+    sq = share_sum(sh, sq);
     if (sh.lane == 0) {
       const float r = rstd_of(sq, (float)s.hw * (float)s.cg, eps);
-      sums[g] = mean;
-      sums[s.g + g] = r;
+      sums[0][sh.group] = mean;
+      sums[1][sh.group] = r;
       if (stat) {
         stat[(int64_t)b * s.g + g] = mean;
         stat[((int64_t)s.b + b) * s.g + g] = r;
@@ -768,10 +798,11 @@ __global__ __launch_bounds__(THREADS) void gn_join(
     }
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < s.c; c += THREADS) {
-    const int g = c / s.cg;
-    chan[(int64_t)b * s.c + c] = sums[g];
-    chan[((int64_t)s.b + b) * s.c + c] = sums[s.g + g] * (w ? w[c] : 1.0f);
+  const int last = min(g0 + sh.groups, s.g) * s.cg;
+  for (int c = g0 * s.cg + threadIdx.x; c < last; c += THREADS) {
+    const int at = small_div(c, s.cg) - g0;
+    chan[(int64_t)b * s.c + c] = sums[0][at];
+    chan[((int64_t)s.b + b) * s.c + c] = sums[1][at] * (w ? w[c] : 1.0f);
   }
 }
 
@@ -882,41 +913,48 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_sums(
         make_float2(joined[g], joined[s.g + g]);
 }
 
-// A block per sample.  chan: [4][b][c], for every channel its mean, rstd w, and
-// what dx adds to rstd w gz: chan2 + (x - mean) chan3.
+// Block (groups, sample).  chan: [4][b][c], for every channel its mean, rstd w,
+// and what dx adds to rstd w gz: chan2 + (x - mean) chan3.
 __global__ __launch_bounds__(THREADS) void gn_bwd_join(
     const float2* __restrict__ part_g, const float* __restrict__ w,
     const float* __restrict__ stat, float* __restrict__ chan, Shape s,
-    Deal deal) {
-  extern __shared__ float sums[];  // [2][g]
-  const int b = blockIdx.x;
-  const Share sh(s.g);
-  const float inv_n = 1.0f / ((float)s.hw * (float)s.cg);
-  const float* mean = stat + (int64_t)b * s.g;
-  const float* rstd = stat + ((int64_t)s.b + b) * s.g;
-  for (int g = sh.group; g < s.g; g += sh.step) {
+    Deal deal, int lanes) {
+  __shared__ float sums[4][THREADS];
+  const Share sh = share_of(lanes, s.g);
+  const int b = blockIdx.x / sh.blocks;
+  const int g0 = (blockIdx.x - b * sh.blocks) * sh.groups;
+  const int g = g0 + sh.group;
+  if (g < s.g) {
+    float2 v[MOST];
+    share_load(sh, part_g + ((int64_t)b * s.g + g) * deal.n, deal.n, v);
+    const float mean = stat[(int64_t)b * s.g + g];
+    const float rstd = stat[((int64_t)s.b + b) * s.g + g];
     float a = 0.0f, c = 0.0f;
-    sh.each(part_g + ((int64_t)b * s.g + g) * deal.n, deal.n,
-            [&](int, float2 v) {
-              a += v.x;
-              c += v.y;
-            });
-    a = sh.sum(a);
-    c = sh.sum(c);
+#pragma unroll
+    for (int q = 0; q < MOST; ++q) {
+      a += v[q].x;
+      c += v[q].y;
+    }
+    a = share_sum(sh, a);
+    c = share_sum(sh, c);
     if (sh.lane == 0) {
-      sums[g] = -rstd[g] * (a * inv_n);
-      sums[s.g + g] = -rstd[g] * rstd[g] * (c * inv_n);
+      const float inv_n = 1.0f / ((float)s.hw * (float)s.cg);
+      sums[0][sh.group] = mean;
+      sums[1][sh.group] = rstd;
+      sums[2][sh.group] = -rstd * (a * inv_n);
+      sums[3][sh.group] = -rstd * rstd * (c * inv_n);
     }
   }
   __syncthreads();
   const int64_t plane = (int64_t)s.b * s.c;
-  for (int c = threadIdx.x; c < s.c; c += THREADS) {
-    const int g = c / s.cg;
+  const int last = min(g0 + sh.groups, s.g) * s.cg;
+  for (int c = g0 * s.cg + threadIdx.x; c < last; c += THREADS) {
+    const int i = small_div(c, s.cg) - g0;
     float* at = chan + (int64_t)b * s.c + c;
-    at[0] = mean[g];
-    at[plane] = rstd[g] * (w ? w[c] : 1.0f);
-    at[2 * plane] = sums[g];
-    at[3 * plane] = sums[s.g + g];
+    at[0] = sums[0][i];
+    at[plane] = sums[1][i] * (w ? w[c] : 1.0f);
+    at[2 * plane] = sums[2][i];
+    at[3 * plane] = sums[3][i];
   }
 }
 
@@ -1068,15 +1106,22 @@ Plan plan_tiles(const Shape& s, int v, size_t value, bool back) {
   return p;
 }
 
+int join_blocks(const Shape& s, int lanes) {
+  const int groups = THREADS / lanes;
+  return (s.g + groups - 1) / groups;
+}
+
 // Blocks per sample that sum: about 512 over the batch, two per CU, with `deep` vectors
-// per thread or more; at most 256, which a join still reads at once.
+// per thread or more; at most what a join reads at once.
 Deal deal_pixels(const Shape& s, int v, int deep) {
   Deal d;
   d.batch = THREADS / std::min(THREADS, s.c / v) * deep;
   d.batches = (int)((s.hw + d.batch - 1) / d.batch);
   d.missing = (int)((int64_t)d.batches * d.batch - s.hw);
-  d.n = std::max(1, std::min({(512 + s.b - 1) / s.b, d.batches, 256}));
-  TORCH_CHECK((int64_t)s.b * d.n < (1ll << 31), "group_norm: tensor too large");
+  d.n = std::max(1, std::min({(512 + s.b - 1) / s.b, d.batches, MOST_PARTS}));
+  // joins have at most as many blocks as a sample has groups
+  TORCH_CHECK((int64_t)s.b * std::max(d.n, s.g) < (1ll << 31),
+              "group_norm: tensor too large");
   return d;
 }
 
@@ -1174,8 +1219,9 @@ void gn_forward(const at::Tensor& x, at::Tensor& y, const float* w,
   hipLaunchKernelGGL(stats, dim3(s.b * deal.n), dim3(THREADS), lds, stream, px,
                      part, s, deal, p.units);
   C10_HIP_KERNEL_LAUNCH_CHECK();
-  hipLaunchKernelGGL(gn_join, dim3(s.b), dim3(THREADS), 8 * s.g, stream, part,
-                     w, stat, chan, s, deal, eps);
+  const int lanes = share_lanes(deal.n);
+  hipLaunchKernelGGL(gn_join, dim3(s.b * join_blocks(s, lanes)), dim3(THREADS),
+                     0, stream, part, w, stat, chan, s, deal, lanes, eps);
   C10_HIP_KERNEL_LAUNCH_CHECK();
   const bool nt = x.numel() * (int64_t)sizeof(T) > STREAM_BYTES;
   GN_VARIANT(v, act, d.on, {
@@ -1237,8 +1283,10 @@ void gn_backward(const at::Tensor& x, const at::Tensor& gy, at::Tensor& dx_out,
                        pg, w, bias, stat, part_c, part_g, s, deal, act, d);
     C10_HIP_KERNEL_LAUNCH_CHECK();
     if (dx) {
-      hipLaunchKernelGGL(gn_bwd_join, dim3(s.b), dim3(THREADS), 8 * s.g, stream,
-                         part_g, w, stat, chan, s, deal);
+      const int lanes = share_lanes(deal.n);
+      hipLaunchKernelGGL(gn_bwd_join, dim3(s.b * join_blocks(s, lanes)),
+                         dim3(THREADS), 0, stream, part_g, w, stat, chan, s,
+                         deal, lanes);
       C10_HIP_KERNEL_LAUNCH_CHECK();
       hipLaunchKernelGGL((gn_bwd_dx<T, V, ACT, DROP>),
                          dim3(s.b * ps.pieces * ps.chunks + param_blocks),
