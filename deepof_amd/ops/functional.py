@@ -246,18 +246,19 @@ def draw_rng(device, generator: torch.Generator | None = None) -> torch.Tensor:
                          generator=generator)
 
 
-def _check_act(act):
-    if act not in _ACT_CODES:
-        raise ValueError(f"unknown activation {act!r}")
+def _act_code(act) -> int:
+    try:
+        return _ACT_CODES[act]
+    except (KeyError, TypeError):
+        raise ValueError(f"unknown activation {act!r}") from None
 
 
 def _check_float(x, name):
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name}: a tensor expected, got {type(x).__name__}")
-    allowed = (torch.float32, torch.float16, torch.bfloat16)
-    if x.dtype not in allowed and (x.is_cuda or x.dtype != torch.float64):
-        raise TypeError(f"{name}: float32, float16 or bfloat16 expected, got "
-                        f"{x.dtype}")
+    allowed = (torch.float64, torch.float32, torch.float16, torch.bfloat16)
+    if x.dtype not in allowed:
+        raise TypeError(f"{name}: a floating tensor expected, got {x.dtype}")
 
 
 def _check_dropout(p, rng, x):
@@ -312,13 +313,15 @@ def dropout(x: torch.Tensor, p: float = 0.5, rng=None,
     p is held to 2^-32.  A captured graph replays the mask of a pair of ints;
     it reads a tensor anew, and draws anew where rng is None.
     """
-    _check_float(x, "dropout")
-    _check_act(act)
+    code = _act_code(act)
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"dropout: a tensor expected, got {type(x).__name__}")
     p, rng, seed, offset = _check_dropout(p, rng, x)
+    if x.is_cuda:  # x is checked by the native call
+        return require_hip().dropout(x, code, p, rng, seed, offset)
+    _check_float(x, "dropout")
     x = x.contiguous(memory_format=_dense_format(x))
-    if not x.is_cuda:
-        return ref.dropout(x, p, _rng_tensor(rng, seed, offset), act)
-    return require_hip().dropout(x, _ACT_CODES[act], p, rng, seed, offset)
+    return ref.dropout(x, p, _rng_tensor(rng, seed, offset), act)
 
 
 def group_norm(x: torch.Tensor, num_groups: int,
@@ -333,14 +336,22 @@ def group_norm(x: torch.Tensor, num_groups: int,
     "elu", "leaky_relu" (0.1), "relu" or "silu".  dropout: its probability;
     rng as for `dropout`, whose mask for the same rng is the same.
     """
+    code = _act_code(act)
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"group_norm: a tensor expected, got "
+                        f"{type(x).__name__}")
+    if type(num_groups) is not int:
+        raise TypeError(f"group_norm: num_groups must be an int, got "
+                        f"{num_groups!r}")
+    p, rng, seed, offset = _check_dropout(dropout, rng, x)
+    if x.is_cuda:  # tensors, groups and eps are checked by the native call
+        return require_hip().group_norm(x, num_groups, weight, bias, eps, code,
+                                        p, rng, seed, offset)
     _check_float(x, "group_norm")
     if x.dim() != 4:
         raise ValueError(f"group_norm: [B, C, H, W] expected, got "
                          f"{tuple(x.shape)}")
     c = x.shape[1]
-    if isinstance(num_groups, bool) or not isinstance(num_groups, int):
-        raise TypeError(f"group_norm: num_groups must be an int, got "
-                        f"{num_groups!r}")
     if not 1 <= num_groups <= _MAX_GROUPS or c == 0 or c % num_groups:
         raise ValueError(f"group_norm: {c} channels in {num_groups} groups "
                          f"(at most {_MAX_GROUPS})")
@@ -351,17 +362,9 @@ def group_norm(x: torch.Tensor, num_groups: int,
         if t.shape != (c,) or t.device != x.device:
             raise ValueError(f"group_norm: {name} must be [{c}] on {x.device}, "
                              f"got {tuple(t.shape)} on {t.device}")
-    if not (eps > 0.0 and eps < float("inf")):
+    if not 0.0 < eps < float("inf"):
         raise ValueError(f"group_norm: eps must be positive, got {eps}")
-    _check_act(act)
-    p, rng, seed, offset = _check_dropout(dropout, rng, x)
     x = x.contiguous(memory_format=torch.channels_last)
-    if not x.is_cuda:
-        y = ref.group_norm(x, num_groups, weight, bias, eps, act, p,
-                           _rng_tensor(rng, seed, offset) if p else None)
-        return y.contiguous(memory_format=torch.channels_last)
-    # the kernels read fp32 parameters; a cast is part of the graph
-    weight = None if weight is None else weight.float().contiguous()
-    bias = None if bias is None else bias.float().contiguous()
-    return require_hip().group_norm(x, num_groups, weight, bias, eps,
-                                    _ACT_CODES[act], p, rng, seed, offset)
+    y = ref.group_norm(x, num_groups, weight, bias, eps, act, p,
+                       _rng_tensor(rng, seed, offset) if p else None)
+    return y.contiguous(memory_format=torch.channels_last)

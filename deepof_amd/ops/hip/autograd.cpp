@@ -5,6 +5,10 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <cmath>
+
+#include "group_norm.h"
+
 using at::Tensor;
 using OptTensor = c10::optional<Tensor>;
 using torch::autograd::AutogradContext;
@@ -86,7 +90,8 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
 };
 
 at::MemoryFormat dense_format(const Tensor& x) {
-  return !x.is_contiguous() && x.is_contiguous(at::MemoryFormat::ChannelsLast)
+  return x.dim() == 4 && !x.is_contiguous() &&
+                 x.is_contiguous(at::MemoryFormat::ChannelsLast)
              ? at::MemoryFormat::ChannelsLast
              : at::MemoryFormat::Contiguous;
 }
@@ -124,24 +129,61 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
 };
 
-bool wanted(const Tensor& t) { return t.defined() && t.requires_grad(); }
+void check_values(const Tensor& x, const char* name) {
+  TORCH_CHECK_TYPE(x.scalar_type() == at::kFloat ||
+                       x.scalar_type() == at::kHalf ||
+                       x.scalar_type() == at::kBFloat16,
+                   name, ": float32, float16 or bfloat16 expected, got ",
+                   x.scalar_type());
+}
+
+// A parameter as the kernels read it: fp32, contiguous.  A cast is part of the
+// graph.
+OptTensor param(const OptTensor& t, const Tensor& x, const char* name) {
+  if (!t.has_value() || !t->defined()) return c10::nullopt;
+  check_values(*t, name);
+  TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == x.size(1) &&
+                        t->device() == x.device(),
+                    name, " must be [", x.size(1), "] on ", x.device(),
+                    ", got ", t->sizes(), " on ", t->device());
+  if (t->scalar_type() == at::kFloat && t->is_contiguous()) return t;
+  return t->to(at::kFloat).contiguous();
+}
 
 }  // namespace
 
-Tensor group_norm(const Tensor& x, int64_t groups, const OptTensor& weight,
+Tensor group_norm(const Tensor& input, int64_t groups, const OptTensor& weight,
                   const OptTensor& bias, double eps, int64_t act, double p,
                   const OptTensor& rng, int64_t seed, int64_t offset) {
-  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
-  if (at::GradMode::is_enabled() && (wanted(x) || wanted(w) || wanted(b)))
-    return GroupNorm::apply(x, weight, bias, groups, eps, act, p, rng, seed,
-                            offset);
-  return group_norm_forward(x, groups, w, b, eps, act, p,
+  check_values(input, "group_norm");
+  TORCH_CHECK_VALUE(input.dim() == 4, "group_norm: [B, C, H, W] expected, got ",
+                    input.sizes());
+  const int64_t c = input.size(1);
+  TORCH_CHECK_VALUE(groups >= 1 && groups <= MAX_GROUPS && c > 0 &&
+                        c % groups == 0,
+                    "group_norm: ", c, " channels in ", groups,
+                    " groups (at most ", MAX_GROUPS, ")");
+  TORCH_CHECK_VALUE((float)eps > 0.0f && std::isfinite(eps),
+                    "group_norm: eps must be positive, got ", eps);
+  const OptTensor w = param(weight, input, "group_norm: weight");
+  const OptTensor b = param(bias, input, "group_norm: bias");
+  const Tensor x = input.contiguous(at::MemoryFormat::ChannelsLast);
+  const auto wanted = [](const OptTensor& t) {
+    return t.has_value() && t->requires_grad();
+  };
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || wanted(w) || wanted(b)))
+    return GroupNorm::apply(x, w, b, groups, eps, act, p, rng, seed, offset);
+  return group_norm_forward(x, groups, w.value_or(Tensor()),
+                            b.value_or(Tensor()), eps, act, p,
                             rng.value_or(Tensor()), seed, offset, false)[0];
 }
 
-Tensor dropout(const Tensor& x, int64_t act, double p, const OptTensor& rng,
+Tensor dropout(const Tensor& input, int64_t act, double p, const OptTensor& rng,
                int64_t seed, int64_t offset) {
-  if (at::GradMode::is_enabled() && wanted(x))
+  check_values(input, "dropout");
+  const Tensor x = input.contiguous(dense_format(input));
+  if (at::GradMode::is_enabled() && x.requires_grad())
     return Dropout::apply(x, act, p, rng, seed, offset);
   return dropout_forward(x, act, p, rng.value_or(Tensor()), seed, offset);
 }

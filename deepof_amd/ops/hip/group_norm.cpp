@@ -7,8 +7,6 @@
 
 namespace {
 
-constexpr int MAX_GROUPS = 4096;  // their sums live in LDS
-
 GroupNormShape shape_of(const at::Tensor& x, int64_t groups) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 4 &&
                   x.is_contiguous(at::MemoryFormat::ChannelsLast),

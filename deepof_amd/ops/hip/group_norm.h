@@ -5,6 +5,8 @@
 
 #include "dropout_args.h"
 
+constexpr int MAX_GROUPS = 4096;  // their sums live in LDS
+
 struct GroupNormShape {
   int64_t hw;
   int b, c, g, cg;  // cg = c / g

@@ -12,7 +12,7 @@ import math
 import torch
 import torch.nn as nn
 
-from .functional import _check_act, dropout, group_norm
+from .functional import _act_code, dropout, group_norm
 
 
 class GroupNormAct(nn.Module):
@@ -32,7 +32,7 @@ class GroupNormAct(nn.Module):
         if not 0.0 <= dropout <= 1.0:
             raise ValueError(f"dropout probability must lie in [0, 1], got "
                              f"{dropout}")
-        _check_act(act)
+        _act_code(act)  # refuses what is none
         self.act, self.eps, self.dropout = act, eps, dropout
         self.weight = nn.Parameter(torch.ones(channels))
         self.bias = nn.Parameter(torch.zeros(channels))
@@ -58,7 +58,7 @@ class CounterDropout(nn.Module):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"dropout probability must lie in [0, 1], got {p}")
-        _check_act(act)
+        _act_code(act)  # refuses what is none
         self.p, self.act = p, act
 
     def forward(self, x):
