@@ -84,7 +84,8 @@ void launch(const void* x, const void* gy, void* out, int64_t n, int act,
             const DropoutArgs& d) {
   const int64_t per_block = (int64_t)BLOCK * UNROLL * 8;
   const int64_t blocks = (n + per_block - 1) / per_block;
-  TORCH_CHECK(blocks < (1ll << 31), "dropout: tensor too large");
+  // a launch's threads are counted in 32 bits
+  TORCH_CHECK(blocks * BLOCK < (1ll << 32), "dropout: tensor too large");
   const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
   auto kernel = dropout_kernel<T, false, BACK, ACT_ANY>;
   if (wide(x) && wide(gy) && wide(out)) {

@@ -109,6 +109,12 @@ __device__ __forceinline__ void each_group(int ch, int cg, F f) {
   }
 }
 
+// Squares that rounding has left below 0; what is no number stays none, so
+// that squares beyond fp32 do not pass for a small variance.
+__device__ __forceinline__ float not_below_0(float v) {
+  return v < 0.0f ? 0.0f : v;
+}
+
 __device__ __forceinline__ float rstd_of(float m2, float n, float eps) {
   return 1.0f / sqrtf(m2 / n + eps);
 }
@@ -236,7 +242,7 @@ struct Moments {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float m = s1[j] * inv;
-      s2[j] = fmaxf(s2[j] - s1[j] * m, 0.0f);
+      s2[j] = not_below_0(s2[j] - s1[j] * m);
       s1[j] = k[j] + m;
     }
   }
@@ -281,7 +287,7 @@ __device__ __forceinline__ void join_moments(Moments<V>& t, int count,
   __syncthreads();
   sum_groups(red, pl, width, first, upg, [&](int g, float2 sum) {
     const float shift = sum.x / n_of(g);
-    fold(g, mean[g] + shift, fmaxf(sum.y - sum.x * shift, 0.0f));
+    fold(g, mean[g] + shift, not_below_0(sum.y - sum.x * shift));
   });
   __syncthreads();
 }
@@ -1065,6 +1071,11 @@ int vector_of(const Shape& s, std::initializer_list<const void*> ptrs) {
   return 1;
 }
 
+// A launch's threads are counted in 32 bits.
+void check_launch(int64_t blocks, int threads) {
+  TORCH_CHECK(blocks * threads < (1ll << 32), "group_norm: tensor too large");
+}
+
 struct Plan {
   bool tiled;
   Tiles tiles;
@@ -1098,7 +1109,6 @@ Plan plan_tiles(const Shape& s, int v, size_t value, bool back) {
         (back ? 4 * RED_CHANNELS(v) + 8 * span : 8 * THREADS * p.units) +
         8 * (span / s.cg);
     if (lds > (int64_t)TILE_LDS) break;
-    if (s.b * spans >= (1ll << 31)) continue;
     p.tiled = true;
     p.lds = (size_t)lds;
     p.tiles = {(int)span, (int)spans, (int)(span / s.cg), (int)iters};
@@ -1120,8 +1130,7 @@ Deal deal_pixels(const Shape& s, int v, int deep) {
   d.missing = (int)((int64_t)d.batches * d.batch - s.hw);
   d.n = std::max(1, std::min({(512 + s.b - 1) / s.b, d.batches, MOST_PARTS}));
   // joins have at most as many blocks as a sample has groups
-  TORCH_CHECK((int64_t)s.b * std::max(d.n, s.g) < (1ll << 31),
-              "group_norm: tensor too large");
+  check_launch((int64_t)s.b * std::max(d.n, s.g), THREADS);
   return d;
 }
 
@@ -1132,8 +1141,7 @@ Pieces cut_pieces(const Shape& s, int v, int deep, int64_t more) {
   p.pixels = BLOCK / cols * deep;
   p.chunks = (s.c / v + BLOCK - 1) / BLOCK;
   p.pieces = (int)((s.hw + p.pixels - 1) / p.pixels);
-  TORCH_CHECK((int64_t)s.b * p.pieces * p.chunks + more < (1ll << 31),
-              "group_norm: tensor too large");
+  check_launch((int64_t)s.b * p.pieces * p.chunks + more, BLOCK);
   return p;
 }
 
@@ -1191,6 +1199,7 @@ void gn_forward(const at::Tensor& x, at::Tensor& y, const float* w,
   const int v = vector_of<T>(s, {px, py});
   const Plan p = plan_tiles(s, v, sizeof(T), false);
   if (p.tiled) {
+    check_launch((int64_t)s.b * p.tiles.spans, THREADS);
     GN_VARIANT(v, act, d.on, {
       auto kernel = gn_tile<T, V, ACT, DROP>;
       allow_lds(kernel, p.lds);
@@ -1245,6 +1254,7 @@ void gn_backward(const at::Tensor& x, const at::Tensor& gy, at::Tensor& dx_out,
   const int param_blocks = db || dw ? (s.c + 7) / 8 : 0;
   const Plan p = plan_tiles(s, v, sizeof(T), true);
   if (p.tiled) {
+    check_launch((int64_t)s.b * p.tiles.spans, THREADS);
     at::Tensor buf;
     float* sums = nullptr;
     if (param_blocks) {

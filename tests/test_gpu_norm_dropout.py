@@ -73,6 +73,8 @@ SHAPES = [  # b, c, h, w, groups
     (2, 256, 1, 40, 8),
     (3, 2048, 4, 5, 16),
     (1, 48, 211, 97, 2),
+    (2, 32, 64, 64, 4),       # a tile of more than 64 KB of LDS
+    (1, 4096, 50, 70, 4096),  # as many groups as there may be, split
 ]
 IDS = ["x".join(map(str, s)) for s in SHAPES]
 
@@ -209,6 +211,45 @@ def test_group_norm_one_gradient_alone(which):
     y = ops.group_norm(leaves[0], 8, leaves[1], leaves[2], act="elu")
     g = torch.autograd.grad(y, leaves[which], gy.to(DEV))[0]
     assert_near(g, want, FP32, magnitudes(x, 8, w, b, gy, 1.0)[1 + which])
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_group_norm_one_gradient_alone_of_a_large_sample(which):
+    x = features((1, 16, 130, 67), FP32, 5)
+    gy = features((1, 16, 130, 67), FP32, 6)
+    w, b = params(16, 5)
+    want = oracle(x, 4, w, b, "elu", gy=gy)[1 + which]
+    leaves = [t.to(DEV) for t in (x, w, b)]
+    leaves[which].requires_grad_(True)
+    y = ops.group_norm(leaves[0], 4, leaves[1], leaves[2], act="elu")
+    g = torch.autograd.grad(y, leaves[which], gy.to(DEV))[0]
+    assert_near(g, want, FP32, magnitudes(x, 4, w, b, gy, 1.0)[1 + which])
+
+
+@pytest.mark.parametrize("hw", [(9, 8), (120, 130)], ids=["tile", "split"])
+def test_group_norm_squares_beyond_fp32(hw):
+    """Finite values whose squares are not: no result that looks like one."""
+    x = features((1, 16) + hw, FP32, 60) * 1e25
+    y = ops.group_norm(x.to(DEV), 4)
+    assert not (torch.isfinite(y) & (y != 0)).any()
+
+
+def test_many_samples_of_one_pixel():
+    x = features((20000, 8, 1, 1), FP32, 61)
+    gy = features((20000, 8, 1, 1), FP32, 62)
+    w, b = params(8, 63)
+    want = oracle(x, 2, w, b, "elu", gy=gy)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+    y = ops.group_norm(leaves[0], 2, *leaves[1:], act="elu")
+    got = (y,) + torch.autograd.grad(y, leaves, gy.to(DEV))
+    for a, t, m in zip(got, want, magnitudes(x, 2, w, b, gy, 1.0)):
+        assert_near(a, t, FP32, m)
+
+
+def test_too_many_samples_are_refused():
+    x = torch.empty(1, 8, 1, 1, device=DEV).expand(9_000_000, -1, -1, -1)
+    with pytest.raises(RuntimeError, match="too large"):
+        ops.group_norm(x, 2)
 
 
 def test_group_norm_16_bit_parameters():
@@ -382,6 +423,14 @@ def test_dropout_mask_and_values(n, dtype):
             assert_near(got, want, dtype, 0.0)
 
 
+def test_dropout_of_any_64_bits():
+    x = torch.ones(5000, device=DEV)
+    for rng in ([-1, -1], [-2**63, 2**63 - 1], [0, 0], [5, -7]):
+        rng = torch.tensor(rng)
+        keep = ref.dropout_keep(x.cpu(), 0.3, rng)
+        assert torch.equal((ops.dropout(x, 0.3, rng.to(DEV)) != 0).cpu(), keep)
+
+
 def test_dropout_undecided_upper_halves():
     """p so placed that the upper 16 bits leave many elements undecided, and
     the lower ones decide: every one of 2^20 elements as the definition says."""
@@ -513,8 +562,9 @@ def test_on_another_stream():
         assert torch.equal(a, t)
 
 
-@pytest.mark.parametrize("shape", [(2, 64, 6, 8), (2, 64, 60, 50)],
-                         ids=["small", "large"])
+@pytest.mark.parametrize("shape", [(2, 64, 6, 8), (2, 64, 60, 50),
+                                   (1, 64, 64, 64), (2, 64, 120, 90)],
+                         ids=["small", "large", "lds", "split"])
 def test_graph_replays(shape):
     """Forward and backward captured; replays between eager work give what the
     eager calls give for the rng that the graph reads."""
