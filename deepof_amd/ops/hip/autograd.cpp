@@ -19,11 +19,11 @@ std::vector<Tensor> group_norm_forward(const Tensor& x, int64_t groups,
                                        const Tensor& bias, double eps,
                                        int64_t act, double p,
                                        const Tensor& rng, int64_t seed,
-                                       int64_t offset, bool keep_stats);
+                                       int64_t offset, bool keep);
 std::vector<Tensor> group_norm_backward(const Tensor& gy, const Tensor& x,
-                                        const Tensor& weight,
+                                        int64_t groups, const Tensor& weight,
                                         const Tensor& bias,
-                                        const Tensor& stats, int64_t act,
+                                        const Tensor& kept, int64_t act,
                                         double p, const Tensor& rng,
                                         int64_t seed, int64_t offset,
                                         bool need_x, bool need_weight,
@@ -62,6 +62,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     auto out = group_norm_forward(x, groups, w, b, eps, act, p, r, seed, offset,
                                   true);
     ctx->save_for_backward({x, w, b, out[1], r});
+    ctx->saved_data["g"] = groups;
     ctx->saved_data["a"] = act;
     ctx->saved_data["p"] = p;
     ctx->saved_data["s"] = seed;
@@ -77,9 +78,10 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       g = group_norm_backward(
-          gy[0].contiguous(at::MemoryFormat::ChannelsLast), s[0], s[1], s[2],
-          s[3], ctx->saved_data["a"].toInt(), ctx->saved_data["p"].toDouble(),
-          s[4], ctx->saved_data["s"].toInt(), ctx->saved_data["o"].toInt(),
+          gy[0].contiguous(at::MemoryFormat::ChannelsLast), s[0],
+          ctx->saved_data["g"].toInt(), s[1], s[2], s[3],
+          ctx->saved_data["a"].toInt(), ctx->saved_data["p"].toDouble(), s[4],
+          ctx->saved_data["s"].toInt(), ctx->saved_data["o"].toInt(),
           ctx->needs_input_grad(0), has_w && ctx->needs_input_grad(1),
           has_b && ctx->needs_input_grad(has_w ? 2 : 1));
     }

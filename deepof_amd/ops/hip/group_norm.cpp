@@ -5,6 +5,8 @@
 
 #include <c10/core/DeviceGuard.h>
 
+#include <algorithm>
+
 namespace {
 
 GroupNormShape shape_of(const at::Tensor& x, int64_t groups) {
@@ -53,11 +55,20 @@ const float* pointer(const at::Tensor& t) {
 
 }  // namespace
 
-// -> y, and stats (mean and rstd, [2, B, G]) where asked for
+// What a forward call keeps for its backward: floats, [2][b][g] mean and rstd,
+// and behind them as many counters as a backward launch may need (a sample's,
+// or a span of channels').
+int64_t stat_floats(const GroupNormShape& s) {
+  return 2 * (int64_t)s.b * s.g;
+}
+
+int counters(const GroupNormShape& s) { return std::max(s.b, s.c); }
+
+// -> y, and what the backward needs where asked for
 std::vector<at::Tensor> group_norm_forward(
     const at::Tensor& x, int64_t groups, const at::Tensor& weight,
     const at::Tensor& bias, double eps, int64_t act, double p,
-    const at::Tensor& rng, int64_t seed, int64_t offset, bool keep_stats) {
+    const at::Tensor& rng, int64_t seed, int64_t offset, bool keep) {
   const GroupNormShape s = shape_of(x, groups);
   TORCH_CHECK(eps > 0.0, "group_norm: eps must be positive");
   c10::DeviceGuard guard(x.device());
@@ -65,27 +76,34 @@ std::vector<at::Tensor> group_norm_forward(
   const at::Tensor wt = param(weight, x, "weight"), bt = param(bias, x, "bias");
   const float *w = pointer(wt), *b = pointer(bt);
   auto y = at::empty_like(x, x.options(), at::MemoryFormat::ChannelsLast);
-  at::Tensor stats;
-  if (keep_stats)
-    stats = at::empty({2, x.size(0), groups}, x.options().dtype(at::kFloat));
-  float* kept = keep_stats ? stats.data_ptr<float>() : nullptr;
+  at::Tensor kept;
+  float* stat = nullptr;
+  uint32_t* counts = nullptr;
+  if (keep) {
+    kept = at::empty({stat_floats(s) + counters(s)},
+                     x.options().dtype(at::kFloat));
+    stat = kept.data_ptr<float>();
+    counts = (uint32_t*)(stat + stat_floats(s));
+  }
   if (x.numel() > 0)
-    GN_TYPE(x.scalar_type(),
-            gn_forward_, (x, y, w, b, kept, s, (float)eps, (int)act, d));
-  return {y, stats};
+    GN_TYPE(x.scalar_type(), gn_forward_,
+            (x, y, w, b, stat, counts, counters(s), s, (float)eps, (int)act, d));
+  return {y, kept};
 }
 
-// -> dx, dweight, dbias; an undefined tensor where none is wanted
+// -> dx, dweight, dbias; an undefined tensor where none is wanted.  The
+// counters in `kept` are used, and left as they were: calls with the same one
+// follow each other on a stream, as the engine has them.
 std::vector<at::Tensor> group_norm_backward(
-    const at::Tensor& gy, const at::Tensor& x, const at::Tensor& weight,
-    const at::Tensor& bias, const at::Tensor& stats, int64_t act, double p,
-    const at::Tensor& rng, int64_t seed, int64_t offset, bool need_x,
-    bool need_weight, bool need_bias) {
-  TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() &&
-                  stats.dim() == 3 && stats.size(0) == 2 &&
-                  stats.size(1) == x.size(0) && stats.device() == x.device(),
-              "group_norm: stats must be [2, B, G] floats");
-  const GroupNormShape s = shape_of(x, stats.size(2));
+    const at::Tensor& gy, const at::Tensor& x, int64_t groups,
+    const at::Tensor& weight, const at::Tensor& bias, const at::Tensor& kept,
+    int64_t act, double p, const at::Tensor& rng, int64_t seed, int64_t offset,
+    bool need_x, bool need_weight, bool need_bias) {
+  const GroupNormShape s = shape_of(x, groups);
+  TORCH_CHECK(kept.scalar_type() == at::kFloat && kept.is_contiguous() &&
+                  kept.numel() == stat_floats(s) + counters(s) &&
+                  kept.device() == x.device(),
+              "group_norm: not what the forward call kept");
   TORCH_CHECK(gy.sizes() == x.sizes() && gy.scalar_type() == x.scalar_type() &&
                   gy.device() == x.device() &&
                   gy.is_contiguous(at::MemoryFormat::ChannelsLast),
@@ -105,8 +123,9 @@ std::vector<at::Tensor> group_norm_backward(
     return {dx, dw, db};
   }
   if (!need_x && !need_weight && !need_bias) return {dx, dw, db};
+  float* stat = kept.data_ptr<float>();
   GN_TYPE(x.scalar_type(), gn_backward_,
-          (x, gy, dx, w, b, stats.data_ptr<float>(),
+          (x, gy, dx, w, b, stat, (uint32_t*)(stat + stat_floats(s)),
            need_bias ? db.data_ptr<float>() : nullptr,
            need_weight ? dw.data_ptr<float>() : nullptr, s, (int)act, d));
   return {dx, dw, db};

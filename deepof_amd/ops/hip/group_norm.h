@@ -12,17 +12,18 @@ struct GroupNormShape {
   int b, c, g, cg;  // cg = c / g
 };
 
-// stat: [2][b][g], mean and rstd; written going forwards unless null.
-// dx, dw, db: null where not wanted.
+// stat: [2][b][g], mean and rstd, and counts, for the way back; both written
+// going forwards unless null.  Going backwards counts are 0 before and after.
+// dx undefined, dw or db null: not wanted.
 #define GN_DECLARE(NAME)                                                      \
   void gn_forward_##NAME(const at::Tensor& x, at::Tensor& y, const float* w,  \
-                         const float* bias, float* stat,                      \
-                         const GroupNormShape& s, float eps, int act,         \
-                         const DropoutArgs& d);                               \
+                         const float* bias, float* stat, uint32_t* counts,    \
+                         int n_counts, const GroupNormShape& s, float eps,    \
+                         int act, const DropoutArgs& d);                      \
   void gn_backward_##NAME(const at::Tensor& x, const at::Tensor& gy,          \
                           at::Tensor& dx, const float* w, const float* bias,  \
-                          const float* stat, float* db, float* dw,            \
-                          const GroupNormShape& s, int act,                   \
+                          const float* stat, uint32_t* counts, float* db,     \
+                          float* dw, const GroupNormShape& s, int act,        \
                           const DropoutArgs& d);
 GN_DECLARE(f32)
 GN_DECLARE(f16)

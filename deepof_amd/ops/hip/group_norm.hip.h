@@ -489,6 +489,58 @@ __device__ __forceinline__ void walk(int count, Load load, Use use) {
 }
 
 // ---------------------------------------------------------------------------
+// the last block
+// ---------------------------------------------------------------------------
+// Blocks that work on one sum leave their parts, and the last of them to come
+// adds all up, in an order that does not depend on which one that is.  Nobody
+// waits.  The parts go through atomics of agent scope, past the L2s that XCDs
+// do not share.  Counters are 0 before a launch: the forward launch has cleared
+// them, and a last block leaves its own at 0 again.
+__device__ __forceinline__ void put2(uint64_t* at, float a, float b) {
+  const uint64_t v =
+      (uint64_t)__float_as_uint(a) | (uint64_t)__float_as_uint(b) << 32;
+  __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ float2 get2(const uint64_t* at) {
+  const uint64_t v =
+      __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((uint32_t)v),
+                     __uint_as_float((uint32_t)(v >> 32)));
+}
+
+// Whether this block is the last of `blocks`.  All its threads call it; their
+// put2 calls are done before it counts.  flag: LDS.
+__device__ __forceinline__ bool last_of(int blocks, uint32_t* count,
+                                        int* flag) {
+  if (blocks == 1) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    return true;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const bool last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED,
+                                             __HIP_MEMORY_SCOPE_AGENT) ==
+                      (uint32_t)(blocks - 1);
+    if (last)
+      __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = last;
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+
+// Every block of a forward launch clears its share of n counters.
+__device__ __forceinline__ void clear_counts(uint32_t* count, int n) {
+  if (!count) return;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
+       i += (int64_t)gridDim.x * blockDim.x)
+    count[i] = 0;
+}
+
+// ---------------------------------------------------------------------------
 // tile route
 // ---------------------------------------------------------------------------
 // Tiles narrower than a cache line share lines with their neighbours.  Block
@@ -512,9 +564,10 @@ template <typename T, int V, int ACT, bool DROP>
 __global__ __launch_bounds__(THREADS, 4) void gn_tile(
     const T* __restrict__ x, T* __restrict__ y, const float* __restrict__ w,
     const float* __restrict__ bias, float* __restrict__ mean_out,
-    float* __restrict__ rstd_out, Shape s, Tiles tiles, int units, float eps,
-    int act, DropoutArgs d) {
+    float* __restrict__ rstd_out, uint32_t* __restrict__ counts, int n_counts,
+    Shape s, Tiles tiles, int units, float eps, int act, DropoutArgs d) {
   extern __shared__ char lds[];
+  clear_counts(counts, n_counts);
   Pack<T, V>* slots = reinterpret_cast<Pack<T, V>*>(lds);
   float2* red = reinterpret_cast<float2*>(slots + tiles.iters * THREADS);
   float* mean = reinterpret_cast<float*>(red + THREADS * units);
@@ -569,14 +622,16 @@ __global__ __launch_bounds__(THREADS, 4) void gn_tile(
 }
 
 // LDS: x's and gy's tiles, red, then floats per channel and per group.
-// sums_c: [2][b][c] of the samples' sums of gz and gz xhat, for the
-// parameters' gradients; null where those are not asked for.
+// sums_c: [b][c] of the samples' sums of gz and gz xhat, which the last block of
+// a span adds up to the parameters' gradients; null where none is asked for.
 template <typename T, int V, int ACT, bool DROP>
 __global__ __launch_bounds__(THREADS, 4) void gn_bwd_tile(
     const T* __restrict__ x, const T* __restrict__ gy, T* __restrict__ dx,
     const float* __restrict__ w, const float* __restrict__ bias,
     const float* __restrict__ mean, const float* __restrict__ rstd,
-    float* __restrict__ sums_c, Shape s, Tiles tiles, int act, DropoutArgs d) {
+    uint64_t* __restrict__ sums_c, uint32_t* __restrict__ counts,
+    float* __restrict__ db, float* __restrict__ dw, Shape s, Tiles tiles,
+    int act, DropoutArgs d) {
   extern __shared__ char lds[];
   Pack<T, V>* slots = reinterpret_cast<Pack<T, V>*>(lds);
   const int slot_g = tiles.iters * THREADS;  // gy's slots behind x's
@@ -585,6 +640,7 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_tile(
   float* sum2 = sum1 + tiles.span;
   float* t1 = sum2 + tiles.span;
   float* t2 = t1 + tiles.groups;
+  int* flag = reinterpret_cast<int*>(t2 + tiles.groups);
   const int at_tile = neighbours_together(blockIdx.x, gridDim.x);
   const int span = at_tile % tiles.spans, b = at_tile / tiles.spans;
   const Place pl(tiles.span / V, THREADS);
@@ -630,28 +686,49 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_tile(
                  t2[g - span * tiles.groups] = -r * r * (c * inv_n);
                });
   if (sums_c)
-    for (int c = threadIdx.x; c < tiles.span; c += THREADS) {
-      sums_c[(int64_t)b * s.c + c0 + c] = sum1[c];
-      sums_c[((int64_t)s.b + b) * s.c + c0 + c] = sum2[c];
-    }
-  if (!dx) return;
+    for (int c = threadIdx.x; c < tiles.span; c += THREADS)
+      put2(sums_c + (int64_t)b * s.c + c0 + c, sum1[c], sum2[c]);
   __syncthreads();
-  if (count == 0) return;
-  float m1[V], m2[V];
-  each_group<V>(pl.col * V, s.cg, [&](int j, int g) {
-    m1[j] = t1[g];
-    m2[j] = t2[g];
-  });
-  for (int i = 0; i < count; ++i) {
-    const int64_t at = from + i * next;
-    float e[V], g[V];
-    through<T, V, ACT, DROP>(k, slots[i * THREADS + threadIdx.x],
-                       slots[slot_g + i * THREADS + threadIdx.x], act, d, st,
-                       (uint64_t)at, e, g);
+  if (dx && count) {
+    float m1[V], m2[V];
+    each_group<V>(pl.col * V, s.cg, [&](int j, int g) {
+      m1[j] = t1[g];
+      m2[j] = t2[g];
+    });
+    for (int i = 0; i < count; ++i) {
+      const int64_t at = from + i * next;
+      float e[V], g[V];
+      through<T, V, ACT, DROP>(k, slots[i * THREADS + threadIdx.x],
+                               slots[slot_g + i * THREADS + threadIdx.x], act,
+                               d, st, (uint64_t)at, e, g);
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      g[j] = fmaf(k.a[j], g[j], fmaf(e[j], m2[j], m1[j]));
-    store_pack<T, V>(dx + at, pack<T, V>(g));
+      for (int j = 0; j < V; ++j)
+        g[j] = fmaf(k.a[j], g[j], fmaf(e[j], m2[j], m1[j]));
+      store_pack<T, V>(dx + at, pack<T, V>(g));
+    }
+  }
+  if (!sums_c || !last_of(s.b, counts + span, flag)) return;
+  // samples dealt in `shares` to threads that lie a span apart
+  const int shares = max(1, small_div(THREADS, tiles.span));
+  const int share = shares > 1 ? small_div(threadIdx.x, tiles.span) : 0;
+  float2* red2 = reinterpret_cast<float2*>(red);
+  for (int c1 = 0; c1 < tiles.span; c1 += THREADS) {
+    const int c = c1 + threadIdx.x - share * tiles.span;
+    const bool in = c < tiles.span && share < shares;
+    float2 sum = make_float2(0.0f, 0.0f);
+    if (in) {
+      const uint64_t* at = sums_c + c0 + c;
+#pragma unroll 8
+      for (int i = share; i < s.b; i += shares) add_to(sum, get2(at + (int64_t)i * s.c));
+    }
+    red2[threadIdx.x] = sum;
+    __syncthreads();
+    if (in && share == 0) {
+      for (int q = 1; q < shares; ++q) add_to(sum, red2[q * tiles.span + c]);
+      if (db) db[c0 + c] = sum.x;
+      if (dw) dw[c0 + c] = sum.y;
+    }
+    __syncthreads();
   }
 }
 
@@ -663,8 +740,10 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_tile(
 // and groups that reach over chunks are joined as they come.
 template <typename T, int V>
 __global__ __launch_bounds__(THREADS, 4) void gn_stats(
-    const T* __restrict__ x, float2* __restrict__ part, Shape s, Deal deal,
+    const T* __restrict__ x, float2* __restrict__ part,
+    uint32_t* __restrict__ counts, int n_counts, Shape s, Deal deal,
     int units) {
+  clear_counts(counts, n_counts);
   constexpr int D = AHEAD1<T>;
   __shared__ float2 red[THREADS * V];
   extern __shared__ float joined[];  // [4][g]: work space, then n, mean, M2
@@ -746,8 +825,8 @@ __device__ __forceinline__ Share share_of(int lanes, int groups) {
   return sh;
 }
 
-__device__ __forceinline__ float share_sum(const Share& sh, float v) {
-  for (int o = sh.lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, WAVE);
+__device__ __forceinline__ float share_sum(int lanes, float v) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, WAVE);
   return v;
 }
 
@@ -786,13 +865,13 @@ __global__ __launch_bounds__(THREADS) void gn_join(
       n[q] = i < deal.n ? (float)deal.pixels(i) : 0.0f;
       sm += n[q] * (v[q].x - ref);
     }
-    const float mean = ref + share_sum(sh, sm) / (float)s.hw;
+    const float mean = ref + share_sum(sh.lanes, sm) / (float)s.hw;
 #pragma unroll
     for (int q = 0; q < MOST; ++q) {
       const float d = v[q].x - mean;
       sq += fmaf(n[q] * (float)s.cg, d * d, v[q].y);
     }
-    sq = share_sum(sh, sq);
+    sq = share_sum(sh.lanes, sq);
     if (sh.lane == 0) {
       const float r = rstd_of(sq, (float)s.hw * (float)s.cg, eps);
       sums[0][sh.group] = mean;
@@ -851,18 +930,23 @@ __global__ __launch_bounds__(BLOCK) void gn_apply(
 
 // Block (split, sample): sums of gz and gz xhat of every channel over the
 // split's pixels.  part_c: [2][b * splits][c]; part_g: [b][g][splits] of the
-// same sums weighted by w and added up over the group.
+// same sums weighted by w and added up over the group, which the sample's last
+// block joins.  chan, where dx is asked for: [4][b][c], for every channel its
+// mean, rstd w, and what dx adds to rstd w gz: chan2 + (x - mean) chan3.
 template <typename T, int V, int ACT, bool DROP>
 __global__ __launch_bounds__(THREADS, 4) void gn_bwd_sums(
     const T* __restrict__ x, const T* __restrict__ gy,
     const float* __restrict__ w, const float* __restrict__ bias,
     const float* __restrict__ stat, float* __restrict__ part_c,
-    float2* __restrict__ part_g, Shape s, Deal deal, int act, DropoutArgs d) {
+    uint64_t* __restrict__ part_g, uint32_t* __restrict__ counts,
+    float* __restrict__ chan, Shape s, Deal deal, int lanes, int act,
+    DropoutArgs d) {
   extern __shared__ float lds_sums[];  // red; [2][channels]; [2][g]
   float* red = lds_sums;
   float* sum1 = red + RED_CHANNELS(V);
   float* sum2 = sum1 + min(THREADS * V, s.c);
   float* joined = sum2 + min(THREADS * V, s.c);
+  int* flag = reinterpret_cast<int*>(joined + 2 * s.g);
   const int split = blockIdx.x % deal.n, b = blockIdx.x / deal.n;
   const DropoutState st = dropout_state(d);
   const float* mean = stat + (int64_t)b * s.g;
@@ -914,53 +998,39 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_sums(
     });
     __syncthreads();
   }
+  if (!chan) return;
+  uint64_t* parts = part_g + (int64_t)b * s.g * deal.n;
   for (int g = threadIdx.x; g < s.g; g += THREADS)
-    part_g[((int64_t)b * s.g + g) * deal.n + split] =
-        make_float2(joined[g], joined[s.g + g]);
-}
-
-// Block (groups, sample).  chan: [4][b][c], for every channel its mean, rstd w,
-// and what dx adds to rstd w gz: chan2 + (x - mean) chan3.
-__global__ __launch_bounds__(THREADS) void gn_bwd_join(
-    const float2* __restrict__ part_g, const float* __restrict__ w,
-    const float* __restrict__ stat, float* __restrict__ chan, Shape s,
-    Deal deal, int lanes) {
-  __shared__ float sums[4][THREADS];
-  const Share sh = share_of(lanes, s.g);
-  const int b = blockIdx.x / sh.blocks;
-  const int g0 = (blockIdx.x - b * sh.blocks) * sh.groups;
-  const int g = g0 + sh.group;
-  if (g < s.g) {
-    float2 v[MOST];
-    share_load(sh, part_g + ((int64_t)b * s.g + g) * deal.n, deal.n, v);
-    const float mean = stat[(int64_t)b * s.g + g];
-    const float rstd = stat[((int64_t)s.b + b) * s.g + g];
-    float a = 0.0f, c = 0.0f;
+    put2(parts + (int64_t)g * deal.n + split, joined[g], joined[s.g + g]);
+  if (!last_of(deal.n, counts + b, flag)) return;
+  const int lane = threadIdx.x & (lanes - 1);
+  const float inv_n = 1.0f / ((float)s.hw * (float)s.cg);
+  for (int g = threadIdx.x / lanes; g < s.g; g += THREADS / lanes) {
+    float2 v[MOST], sum = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int q = 0; q < MOST; ++q) {
-      a += v[q].x;
-      c += v[q].y;
+      const int i = lane + q * lanes;
+      v[q] = i < deal.n ? get2(parts + (int64_t)g * deal.n + i)
+                        : make_float2(0.0f, 0.0f);
     }
-    a = share_sum(sh, a);
-    c = share_sum(sh, c);
-    if (sh.lane == 0) {
-      const float inv_n = 1.0f / ((float)s.hw * (float)s.cg);
-      sums[0][sh.group] = mean;
-      sums[1][sh.group] = rstd;
-      sums[2][sh.group] = -rstd * (a * inv_n);
-      sums[3][sh.group] = -rstd * rstd * (c * inv_n);
+#pragma unroll
+    for (int q = 0; q < MOST; ++q) add_to(sum, v[q]);
+    sum.x = share_sum(lanes, sum.x);
+    sum.y = share_sum(lanes, sum.y);
+    if (lane == 0) {
+      joined[g] = -rstd[g] * (sum.x * inv_n);
+      joined[s.g + g] = -rstd[g] * rstd[g] * (sum.y * inv_n);
     }
   }
   __syncthreads();
   const int64_t plane = (int64_t)s.b * s.c;
-  const int last = min(g0 + sh.groups, s.g) * s.cg;
-  for (int c = g0 * s.cg + threadIdx.x; c < last; c += THREADS) {
-    const int i = small_div(c, s.cg) - g0;
+  for (int c = threadIdx.x; c < s.c; c += THREADS) {
+    const int g = small_div(c, s.cg);
     float* at = chan + (int64_t)b * s.c + c;
-    at[0] = sums[0][i];
-    at[plane] = sums[1][i] * (w ? w[c] : 1.0f);
-    at[2 * plane] = sums[2][i];
-    at[3 * plane] = sums[3][i];
+    at[0] = mean[g];
+    at[plane] = rstd[g] * (w ? w[c] : 1.0f);
+    at[2 * plane] = joined[g];
+    at[3 * plane] = joined[s.g + g];
   }
 }
 
@@ -1106,7 +1176,7 @@ Plan plan_tiles(const Shape& s, int v, size_t value, bool back) {
     const int64_t iters = (s.hw + rows - 1) / rows;
     const int64_t lds =
         iters * THREADS * v * (int64_t)value * (back ? 2 : 1) +
-        (back ? 4 * RED_CHANNELS(v) + 8 * span : 8 * THREADS * p.units) +
+        (back ? 4 * RED_CHANNELS(v) + 8 * span + 4 : 8 * THREADS * p.units) +
         8 * (span / s.cg);
     if (lds > (int64_t)TILE_LDS) break;
     p.tiled = true;
@@ -1185,14 +1255,14 @@ void allow_lds(K kernel, size_t bytes) {
   if (bytes > 64 * 1024)
     C10_HIP_CHECK(hipFuncSetAttribute(
         reinterpret_cast<const void*>(kernel),
-        hipFuncAttributeMaxDynamicSharedMemorySize, (int)TILE_LDS));
+        hipFuncAttributeMaxDynamicSharedMemorySize,
+        (int)std::max(bytes, TILE_LDS)));
 }
 
-// stat: [2][b][g] mean and rstd, left for the way back; null: not kept.
 template <typename T>
 void gn_forward(const at::Tensor& x, at::Tensor& y, const float* w,
-             const float* bias, float* stat, const Shape& s, float eps, int act,
-             const DropoutArgs& d) {
+                const float* bias, float* stat, uint32_t* counts, int n_counts,
+                const Shape& s, float eps, int act, const DropoutArgs& d) {
   const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
   const T* px = (const T*)x.data_ptr();
   T* py = (T*)y.data_ptr();
@@ -1200,13 +1270,13 @@ void gn_forward(const at::Tensor& x, at::Tensor& y, const float* w,
   const Plan p = plan_tiles(s, v, sizeof(T), false);
   if (p.tiled) {
     check_launch((int64_t)s.b * p.tiles.spans, THREADS);
+    float* rstd = stat ? stat + (int64_t)s.b * s.g : nullptr;
     GN_VARIANT(v, act, d.on, {
       auto kernel = gn_tile<T, V, ACT, DROP>;
       allow_lds(kernel, p.lds);
       hipLaunchKernelGGL(kernel, dim3(s.b * p.tiles.spans), dim3(THREADS),
-                         p.lds, stream, px, py, w, bias, stat, stat ? stat +
-                         (int64_t)s.b * s.g : nullptr, s, p.tiles, p.units,
-                         eps, act, d);
+                         p.lds, stream, px, py, w, bias, stat, rstd, counts,
+                         n_counts, s, p.tiles, p.units, eps, act, d);
       C10_HIP_KERNEL_LAUNCH_CHECK();
     });
     return;
@@ -1216,8 +1286,7 @@ void gn_forward(const at::Tensor& x, at::Tensor& y, const float* w,
   const int64_t parts = (int64_t)s.b * s.g * deal.n;
   const int64_t plane = (int64_t)s.b * s.c;
   // channels' values first: their vectors are aligned
-  auto buf = at::empty({2 * plane + 2 * parts + 2},
-                       x.options().dtype(at::kFloat));
+  auto buf = at::empty({2 * plane + 2 * parts}, x.options().dtype(at::kFloat));
   float* chan = buf.data_ptr<float>();
   float2* part = (float2*)(chan + 2 * plane);
   const auto stats = v == 8   ? gn_stats<T, 8>
@@ -1226,7 +1295,7 @@ void gn_forward(const at::Tensor& x, at::Tensor& y, const float* w,
   const size_t lds = 4 * (size_t)s.g * 4;
   allow_lds(stats, lds + THREADS * v * 8);
   hipLaunchKernelGGL(stats, dim3(s.b * deal.n), dim3(THREADS), lds, stream, px,
-                     part, s, deal, p.units);
+                     part, counts, n_counts, s, deal, p.units);
   C10_HIP_KERNEL_LAUNCH_CHECK();
   const int lanes = share_lanes(deal.n);
   hipLaunchKernelGGL(gn_join, dim3(s.b * join_blocks(s, lanes)), dim3(THREADS),
@@ -1243,61 +1312,55 @@ void gn_forward(const at::Tensor& x, at::Tensor& y, const float* w,
 
 template <typename T>
 void gn_backward(const at::Tensor& x, const at::Tensor& gy, at::Tensor& dx_out,
-                 const float* w, const float* bias, const float* stat, float* db, float* dw,
-              const Shape& s, int act, const DropoutArgs& d) {
+                 const float* w, const float* bias, const float* stat,
+                 uint32_t* counts, float* db, float* dw, const Shape& s,
+                 int act, const DropoutArgs& d) {
   const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
   const T* px = (const T*)x.data_ptr();
   const T* pg = (const T*)gy.data_ptr();
   T* dx = dx_out.defined() ? (T*)dx_out.data_ptr() : nullptr;
   const int v = vector_of<T>(s, {px, pg, dx});
   const auto opts = x.options().dtype(at::kFloat);
-  const int param_blocks = db || dw ? (s.c + 7) / 8 : 0;
   const Plan p = plan_tiles(s, v, sizeof(T), true);
   if (p.tiled) {
     check_launch((int64_t)s.b * p.tiles.spans, THREADS);
     at::Tensor buf;
-    float* sums = nullptr;
-    if (param_blocks) {
+    uint64_t* sums = nullptr;
+    if (db || dw) {
       buf = at::empty({2 * (int64_t)s.b * s.c}, opts);
-      sums = buf.data_ptr<float>();
+      sums = (uint64_t*)buf.data_ptr();
     }
+    const float* rstd = stat + (int64_t)s.b * s.g;
     GN_VARIANT(v, act, d.on, {
       auto kernel = gn_bwd_tile<T, V, ACT, DROP>;
       allow_lds(kernel, p.lds);
       hipLaunchKernelGGL(kernel, dim3(s.b * p.tiles.spans), dim3(THREADS),
-                         p.lds, stream, px, pg, dx, w, bias, stat, stat +
-                         (int64_t)s.b * s.g, sums, s, p.tiles, act, d);
+                         p.lds, stream, px, pg, dx, w, bias, stat, rstd, sums,
+                         counts, db, dw, s, p.tiles, act, d);
       C10_HIP_KERNEL_LAUNCH_CHECK();
     });
-    if (param_blocks) {
-      hipLaunchKernelGGL(gn_param_grad, dim3(param_blocks), dim3(BLOCK), 0,
-                         stream, sums, s.b, s.c, db, dw);
-      C10_HIP_KERNEL_LAUNCH_CHECK();
-    }
     return;
   }
+  const int param_blocks = db || dw ? (s.c + 7) / 8 : 0;
   const Deal deal = deal_pixels(s, v, AHEAD2<T>);
   const Pieces ps = cut_pieces(s, v, 2 * AHEAD2<T>, param_blocks);
   const int64_t rows = (int64_t)s.b * deal.n, plane = (int64_t)s.b * s.c;
-  auto buf = at::empty({4 * plane + 2 * rows * (s.c + s.g) + 2}, opts);
+  auto buf = at::empty({4 * plane + 2 * rows * (s.c + s.g)}, opts);
   float* chan = buf.data_ptr<float>();
   float* part_c = chan + 4 * plane;
-  float2* part_g = (float2*)(part_c + 2 * rows * s.c);
+  uint64_t* part_g = (uint64_t*)(part_c + 2 * rows * s.c);
   const bool nt = x.numel() * (int64_t)sizeof(T) > STREAM_BYTES;
   GN_VARIANT(v, act, d.on, {
     auto sums = gn_bwd_sums<T, V, ACT, DROP>;
-    const size_t lds =
-        4 * (RED_CHANNELS(V) + 2 * (size_t)std::min(THREADS * V, s.c) + 2 * s.g);
+    const size_t lds = 4 * (RED_CHANNELS(V) +
+                            2 * (size_t)std::min(THREADS * V, s.c) + 2 * s.g + 1);
     allow_lds(sums, lds);
     hipLaunchKernelGGL(sums, dim3(s.b * deal.n), dim3(THREADS), lds, stream, px,
-                       pg, w, bias, stat, part_c, part_g, s, deal, act, d);
+                       pg, w, bias, stat, part_c, part_g, counts,
+                       dx ? chan : nullptr, s, deal, share_lanes(deal.n), act,
+                       d);
     C10_HIP_KERNEL_LAUNCH_CHECK();
     if (dx) {
-      const int lanes = share_lanes(deal.n);
-      hipLaunchKernelGGL(gn_bwd_join, dim3(s.b * join_blocks(s, lanes)),
-                         dim3(THREADS), 0, stream, part_g, w, stat, chan, s,
-                         deal, lanes);
-      C10_HIP_KERNEL_LAUNCH_CHECK();
       hipLaunchKernelGGL((gn_bwd_dx<T, V, ACT, DROP>),
                          dim3(s.b * ps.pieces * ps.chunks + param_blocks),
                          dim3(BLOCK), 0, stream, px, pg, dx, chan, bias, part_c,

@@ -359,6 +359,32 @@ def test_group_norm_is_the_same_every_time():
             assert torch.equal(a, t)
 
 
+@pytest.mark.parametrize("shape", [(8, 64, 6, 8), (4, 64, 120, 90)],
+                         ids=["tile", "split"])
+def test_group_norm_backward_again_and_again(shape):
+    """One graph's backward several times, as a whole and in part, and from
+    saved tensors that were moved to the host and back."""
+    x = features(shape, BF16, 70).to(DEV).requires_grad_(True)
+    w, b = (t.to(DEV).requires_grad_(True) for t in params(64, 71))
+    gy = features(shape, BF16, 72).to(DEV)
+    y = ops.group_norm(x, 8, w, b, act="silu", dropout=0.2, rng=(1, 2))
+    want = torch.autograd.grad(y, (x, w, b), gy, retain_graph=True)
+    for _ in range(3):
+        got = torch.autograd.grad(y, (x, w, b), gy, retain_graph=True)
+        for a, t in zip(got, want):
+            assert torch.equal(a, t)
+        assert torch.equal(
+            torch.autograd.grad(y, w, gy, retain_graph=True)[0], want[1])
+        assert torch.equal(
+            torch.autograd.grad(y, x, gy, retain_graph=True)[0], want[0])
+    with torch.autograd.graph.save_on_cpu():
+        y = ops.group_norm(x, 8, w, b, act="silu", dropout=0.2, rng=(1, 2))
+    for _ in range(2):
+        got = torch.autograd.grad(y, (x, w, b), gy, retain_graph=True)
+        for a, t in zip(got, want):
+            assert torch.equal(a, t)
+
+
 def test_group_norm_against_differences():
     x = features((2, 16, 9, 8), FP32, 16)
     w, b = params(16, 7)
