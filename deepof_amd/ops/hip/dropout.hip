@@ -5,6 +5,15 @@
 //
 // kept(i) is computed from (seed, offset, i) in both directions
 // (philox.hip.h), so neither a mask is written nor read back.
+//
+// Memory bounds it: 64x64x192x256 bf16, 403 MB read and 403 MB written, takes
+// 131 us each way (6.2 TB/s; a plain copy here takes 134 to 148).  The
+// generator costs some 20 quarter-rate products and 100 other instructions per
+// 8 elements, about 90 us of the vector units, which hide behind other waves'
+// loads as long as those are many: at 180 registers a thread, with four vectors
+// in flight, it took 289 us, at 44 with two 193, and 131 once what is larger
+// than the L2s went past the caches.  One short pass per block, blocks in
+// memory's order.
 
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPException.h>

@@ -87,7 +87,8 @@ std::vector<at::Tensor> group_norm_forward(
   }
   if (x.numel() > 0)
     GN_TYPE(x.scalar_type(), gn_forward_,
-            (x, y, w, b, stat, counts, counters(s), s, (float)eps, (int)act, d));
+            (x, y, w, b, stat, counts, counters(s), s, (float)eps, (int)act,
+             d));
   return {y, kept};
 }
 
@@ -114,7 +115,8 @@ std::vector<at::Tensor> group_norm_backward(
   const float *w = pointer(wt), *b = pointer(bt);
   at::Tensor dx, dw, db;
   const auto opts = x.options().dtype(at::kFloat);
-  if (need_x) dx = at::empty_like(x, x.options(), at::MemoryFormat::ChannelsLast);
+  if (need_x)
+    dx = at::empty_like(x, x.options(), at::MemoryFormat::ChannelsLast);
   if (need_weight) dw = at::empty({x.size(1)}, opts);
   if (need_bias) db = at::empty({x.size(1)}, opts);
   if (x.numel() == 0) {

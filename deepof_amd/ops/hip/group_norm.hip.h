@@ -19,15 +19,22 @@
 // Memory bounds all of it.  Two routes:
 //  - tile: where a bundle of whole groups of a sample fits into half a CU's
 //    LDS, a block keeps it there, so that x (and gy) are read once, in one
-//    launch;
-//  - split: else pixels are split over blocks, which leave partial sums; a
-//    small launch joins them, and the last one reads x (and gy) again.
+//    launch each way;
+//  - split: else pixels are dealt to blocks, which leave partial sums, and the
+//    last launch reads x (and gy) again: three launches forwards (sums, their
+//    join, y), two backwards (sums, whose last blocks join them; dx).
+// 64x64x192x256 bf16 with ELU (403 MB a tensor; 1.6 GB is the least that
+// forward and backward move, 3.2 GB is what the split route does): sums 119 us,
+// join 5, y 118; sums 196, dx 182: 5.2 TB/s over all, what a large copy reaches
+// here.  8x24x32x512 bf16 (tile; 6.3 MB): 9.7 us forwards, 13.2 backwards, most
+// of it launch, first loads and the sums' three meetings in LDS.
 // Keeping larger samples on the chip, a team of blocks each with its tile, was
 // built and measured too: a team's meeting costs its blocks some 20 us, in
 // which a CU's LDS holds far less than memory moves, and 64x64x192x256 bf16
-// took 390 us forwards against 290.
+// took 390 us forwards against 290 of the split route then.
 //
-// Sums have a fixed order everywhere: no atomics, equal results every time.
+// Sums have a fixed order everywhere, whichever block ends them: results are
+// equal every time.
 
 #pragma once
 
@@ -513,13 +520,9 @@ __device__ __forceinline__ float2 get2(const uint64_t* at) {
 // put2 calls are done before it counts.  flag: LDS.
 __device__ __forceinline__ bool last_of(int blocks, uint32_t* count,
                                         int* flag) {
-  if (blocks == 1) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    return true;
-  }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
+  if (blocks == 1) return true;
   if (threadIdx.x == 0) {
     const bool last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED,
                                              __HIP_MEMORY_SCOPE_AGENT) ==
@@ -546,7 +549,7 @@ __device__ __forceinline__ void clear_counts(uint32_t* count, int n) {
 // Tiles narrower than a cache line share lines with their neighbours.  Block
 // i's tile is so chosen that neighbours go to the same XCD, whose L2 then
 // fetches a line once, and writes it back whole.  (8x24x32x512 bf16, spans of
-// 32 bytes: 12.0 us without, and see gn_tile with.)
+// 32 bytes: forwards 12.0 us without and 9.2 with, backwards 16.2 and 11.4.)
 __device__ __forceinline__ int neighbours_together(int i, int n) {
   const int each = n / XCDS;
   return i < each * XCDS ? (i % XCDS) * each + i / XCDS : i;
@@ -622,8 +625,8 @@ __global__ __launch_bounds__(THREADS, 4) void gn_tile(
 }
 
 // LDS: x's and gy's tiles, red, then floats per channel and per group.
-// sums_c: [b][c] of the samples' sums of gz and gz xhat, which the last block of
-// a span adds up to the parameters' gradients; null where none is asked for.
+// sums_c: [b][c] of the samples' sums of gz and gz xhat, which the last block
+// of a span adds up to the parameters' gradients; null: none is asked for.
 template <typename T, int V, int ACT, bool DROP>
 __global__ __launch_bounds__(THREADS, 4) void gn_bwd_tile(
     const T* __restrict__ x, const T* __restrict__ gy, T* __restrict__ dx,
@@ -719,7 +722,8 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_tile(
     if (in) {
       const uint64_t* at = sums_c + c0 + c;
 #pragma unroll 8
-      for (int i = share; i < s.b; i += shares) add_to(sum, get2(at + (int64_t)i * s.c));
+      for (int i = share; i < s.b; i += shares)
+        add_to(sum, get2(at + (int64_t)i * s.c));
     }
     red2[threadIdx.x] = sum;
     __syncthreads();
@@ -841,9 +845,9 @@ __device__ __forceinline__ void share_load(const Share& sh, const float2* e,
 }
 
 // Block (groups, sample): joins the splits' statistics, the mean first, about
-// split 0's, then squares about it.  stat: [2][b][g] mean and rstd, kept for the
-// way back, or null.  chan: [2][b][c], mean and rstd w of every channel, which
-// the next launch's threads load as vectors.
+// split 0's, then squares about it.  stat: [2][b][g] mean and rstd, kept for
+// the way back, or null.  chan: [2][b][c], mean and rstd w of every channel,
+// which the next launch's threads load as vectors.
 __global__ __launch_bounds__(THREADS) void gn_join(
     const float2* __restrict__ part, const float* __restrict__ w,
     float* __restrict__ stat, float* __restrict__ chan, Shape s, Deal deal,
@@ -922,9 +926,10 @@ __global__ __launch_bounds__(BLOCK) void gn_apply(
     return load_pack<T, V>(x + from + (in ? i * next : 0), stream);
   }, [&](int i, const Pack<T, V>& raw) {
     const int64_t at = from + i * next;
-    store_pack<T, V>(
-        y + at, forward_value<T, V, ACT, DROP>(k, raw, act, d, st, (uint64_t)at),
-        stream);
+    store_pack<T, V>(y + at,
+                     forward_value<T, V, ACT, DROP>(k, raw, act, d, st,
+                                                    (uint64_t)at),
+                     stream);
   });
 }
 
@@ -1191,8 +1196,9 @@ int join_blocks(const Shape& s, int lanes) {
   return (s.g + groups - 1) / groups;
 }
 
-// Blocks per sample that sum: about 512 over the batch, two per CU, with `deep` vectors
-// per thread or more; at most what a join reads at once.
+// Blocks per sample that sum: about 512 over the batch, two per CU
+// (4x55x128x256 fp32: 1024 of them took 20 us, 512 12), with `deep` vectors per
+// thread or more; at most what a join reads at once.
 Deal deal_pixels(const Shape& s, int v, int deep) {
   Deal d;
   d.batch = THREADS / std::min(THREADS, s.c / v) * deep;
@@ -1352,8 +1358,8 @@ void gn_backward(const at::Tensor& x, const at::Tensor& gy, at::Tensor& dx_out,
   const bool nt = x.numel() * (int64_t)sizeof(T) > STREAM_BYTES;
   GN_VARIANT(v, act, d.on, {
     auto sums = gn_bwd_sums<T, V, ACT, DROP>;
-    const size_t lds = 4 * (RED_CHANNELS(V) +
-                            2 * (size_t)std::min(THREADS * V, s.c) + 2 * s.g + 1);
+    const size_t lds = 4 * (RED_CHANNELS(V) + 2 * s.g + 1 +
+                            2 * (size_t)std::min(THREADS * V, s.c));
     allow_lds(sums, lds);
     hipLaunchKernelGGL(sums, dim3(s.b * deal.n), dim3(THREADS), lds, stream, px,
                        pg, w, bias, stat, part_c, part_g, counts,

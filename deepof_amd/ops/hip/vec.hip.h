@@ -139,7 +139,8 @@ __device__ __forceinline__ void act_apply(int act, float (&v)[V]) {
   switch (ACT == ACT_ANY ? act : ACT) {
     case ACT_ELU:
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[k] = v[k] <= 0.0f ? expm1_neg<T>(v[k]) : v[k];
+      for (int k = 0; k < V; ++k)
+        v[k] = v[k] <= 0.0f ? expm1_neg<T>(v[k]) : v[k];
       break;
     case ACT_LEAKY:
 #pragma unroll
