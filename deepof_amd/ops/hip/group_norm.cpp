@@ -4,6 +4,7 @@
 #include "group_norm.h"
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 
 #include <algorithm>
 
@@ -94,7 +95,9 @@ std::vector<at::Tensor> group_norm_forward(
 
 // -> dx, dweight, dbias; an undefined tensor where none is wanted.  The
 // counters in `kept` are used, and left as they were: calls with the same one
-// follow each other on a stream, as the engine has them.
+// follow each other on a stream, as the engine has them.  Replays of a graph
+// follow nothing, so a call that is being recorded has counters of its own,
+// cleared by a launch of some 2 us in the graph.
 std::vector<at::Tensor> group_norm_backward(
     const at::Tensor& gy, const at::Tensor& x, int64_t groups,
     const at::Tensor& weight, const at::Tensor& bias, const at::Tensor& kept,
@@ -126,8 +129,15 @@ std::vector<at::Tensor> group_norm_backward(
   }
   if (!need_x && !need_weight && !need_bias) return {dx, dw, db};
   float* stat = kept.data_ptr<float>();
+  uint32_t* counts = (uint32_t*)(stat + stat_floats(s));
+  at::Tensor own;
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() !=
+      c10::hip::CaptureStatus::None) {
+    own = at::empty({counters(s)}, x.options().dtype(at::kInt)).zero_();
+    counts = (uint32_t*)own.data_ptr<int>();
+  }
   GN_TYPE(x.scalar_type(), gn_backward_,
-          (x, gy, dx, w, b, stat, (uint32_t*)(stat + stat_floats(s)),
+          (x, gy, dx, w, b, stat, counts,
            need_bias ? db.data_ptr<float>() : nullptr,
            need_weight ? dw.data_ptr<float>() : nullptr, s, (int)act, d));
   return {dx, dw, db};

@@ -622,6 +622,43 @@ def test_graph_replays(shape):
             assert torch.equal(a, t)
 
 
+@pytest.mark.parametrize("shape", [(4, 64, 24, 32, 16), (2, 64, 160, 200, 32)])
+def test_two_graphs_of_one_backward(shape):
+    """Backwards of one call, recorded twice and replayed side by side with
+    eager ones, share no counter."""
+    b, c, h, w, groups = shape
+    side = [torch.cuda.Stream(DEV) for _ in range(3)]
+    x = features((b, c, h, w), BF16, 70).to(DEV).requires_grad_()
+    weight, bias = (t.to(DEV).requires_grad_() for t in params(c, 70))
+    leaves = (x, weight, bias)
+    gys = [features((b, c, h, w), BF16, 71 + i).to(DEV) for i in range(3)]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    with torch.cuda.stream(side[0]):
+        y = ops.group_norm(x, groups, weight, bias, act="elu")
+        want = [torch.autograd.grad(y, leaves, gy, retain_graph=True)
+                for gy in gys]
+    torch.cuda.synchronize()
+    for gy in gys[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side[0]):
+            outs.append(torch.autograd.grad(y, leaves, gy, retain_graph=True))
+        graphs.append(g)
+    for _ in range(20):
+        for out in outs:
+            for t in out:
+                t.fill_(7.0)
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, side[1:]):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(side[0]):
+            eager = torch.autograd.grad(y, leaves, gys[2], retain_graph=True)
+        torch.cuda.synchronize()
+        for got, exact in zip([*outs, eager], want):
+            assert all(torch.equal(a, e) for a, e in zip(got, exact))
+
+
 def test_graph_draws_anew_at_every_replay():
     x = torch.ones(4096, device=DEV)
     ops.dropout(x, 0.5)
