@@ -2,6 +2,7 @@
 64 bits."""
 
 import math
+import threading
 
 import pytest
 import torch
@@ -385,6 +386,21 @@ def test_group_norm_backward_again_and_again(shape):
             assert torch.equal(a, t)
 
 
+@pytest.mark.parametrize("shape", [(2, 32, 7, 9, 8), (2, 64, 90, 120, 16)])
+def test_group_norm_one_tensor_as_weight_and_bias(shape):
+    b, c, h, w, groups = shape
+    x = features((b, c, h, w), BF16, 80).to(DEV).requires_grad_()
+    gy = features((b, c, h, w), BF16, 81).to(DEV)
+    both = params(c, 80)[0].to(DEV).requires_grad_()
+    one, two = (both.detach().clone().requires_grad_() for _ in range(2))
+    y = ops.group_norm(x, groups, both, both, act="silu")
+    dx, d = torch.autograd.grad(y, (x, both), gy)
+    y2 = ops.group_norm(x, groups, one, two, act="silu")
+    dx2, d1, d2 = torch.autograd.grad(y2, (x, one, two), gy)
+    assert torch.equal(y, y2) and torch.equal(dx, dx2)
+    assert torch.equal(d, d1 + d2)
+
+
 def test_group_norm_against_differences():
     x = features((2, 16, 9, 8), FP32, 16)
     w, b = params(16, 7)
@@ -620,6 +636,48 @@ def test_graph_replays(shape):
         torch.cuda.synchronize()
         for a, t in zip(out, want):
             assert torch.equal(a, t)
+
+
+def test_two_threads_at_once():
+    """Calls of two host threads on streams of their own give what they give
+    one after the other."""
+    cases = [(4, 64, 24, 32, 16), (2, 64, 160, 200, 32)]
+    data = []
+    for k, (b, c, h, w, groups) in enumerate(cases):
+        data.append((groups, features((b, c, h, w), BF16, 90 + k).to(DEV),
+                     *(t.to(DEV) for t in params(c, 90 + k)),
+                     features((b, c, h, w), BF16, 95 + k).to(DEV)))
+
+    def calls(k):
+        groups, x, weight, bias, gy = data[k]
+        leaves = [t.detach().requires_grad_() for t in (x, weight, bias)]
+        y = ops.group_norm(leaves[0], groups, *leaves[1:], act="elu",
+                           dropout=0.3, rng=(7, k))
+        z = ops.dropout(y, 0.2, rng=(8, k), act="relu")
+        return [y.detach(), z.detach(), *torch.autograd.grad(z, leaves, gy)]
+
+    want = [calls(k) for k in range(2)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream(DEV)):
+                for i in range(20):
+                    got = calls(k)
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(g, e)
+                               for g, e in zip(got, want[k])):
+                        wrong.append((k, i))
+        except Exception as e:  # a thread's error would be lost
+            wrong.append((k, repr(e)))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 @pytest.mark.parametrize("shape", [(4, 64, 24, 32, 16), (2, 64, 160, 200, 32)])
