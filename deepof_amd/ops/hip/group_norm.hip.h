@@ -221,37 +221,63 @@ __device__ __forceinline__ void sum_groups(const F* red, const Place& pl,
   }
 }
 
-// A thread's sum and sum of squares of its values, per channel, about its
-// first value: a mean far from 0 costs no digits, and a first value far from
-// the others costs no more than it adds to the variance itself.
+// A thread's mean and squares about it, per channel.  Values are summed in runs
+// about what the mean was before the run, the first about the thread's first
+// value, and the runs are joined: a mean far from 0 costs no digits, as
+// differences alone are summed.  The first value may itself lie far from all
+// others, so the first run is short, and later ones are about a mean that has
+// left it behind.  (One sum of squares about the first value adds up nearly
+// equal numbers then, whose roundings all go one way: of 768 values, 0 but for
+// the first, it had the variance wrong by 2e-2, and this by 1e-6.)
+constexpr int FIRST_RUN = 8, RUN = 64;  // multiples of what walk loads ahead
+
 template <int V>
 struct Moments {
-  float k[V], s1[V], s2[V];
+  float mean[V], rest[V];  // the mean is their sum: rest is mean's rounding
+  float m2[V];             // squares about it
+  float s1[V], s2[V];      // of the run, about mean
+  int n, run;              // values joined, and in the run
   __device__ __forceinline__ void begin() {
+    n = run = 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) k[j] = s1[j] = s2[j] = 0.0f;
+    for (int j = 0; j < V; ++j)
+      mean[j] = rest[j] = m2[j] = s1[j] = s2[j] = 0.0f;
   }
   __device__ __forceinline__ void about(const float (&v)[V]) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) k[j] = v[j];
+    for (int j = 0; j < V; ++j) mean[j] = v[j];
   }
   __device__ __forceinline__ void add(const float (&v)[V]) {
+    ++run;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float d = v[j] - k[j];
+      const float d = v[j] - mean[j];
       s1[j] += d;
       s2[j] = fmaf(d, d, s2[j]);
     }
   }
-  // (s1, s2) -> (mean, squares about it) of n values
-  __device__ __forceinline__ void close(float n) {
-    const float inv = 1.0f / n;
+  __device__ __forceinline__ void join() {
+    if (run == 0) return;
+    const float a = (float)n, b = (float)run;
+    const float inv = __builtin_amdgcn_rcpf(b);
+    const float share = b * __builtin_amdgcn_rcpf(a + b);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float m = s1[j] * inv;
-      s2[j] = not_below_0(s2[j] - s1[j] * m);
-      s1[j] = k[j] + m;
+      const float e = s1[j] * inv;     // the run's mean, less mean
+      const float d = e - rest[j];     // less the mean before it
+      m2[j] += fmaf(d * d, a * share, not_below_0(s2[j] - s1[j] * e));
+      const float t = fmaf(d, share, rest[j]);
+      const float m = mean[j] + t;
+      rest[j] = t - (m - mean[j]);
+      mean[j] = m;
+      s1[j] = s2[j] = 0.0f;
     }
+    n += run;
+    run = 0;
+  }
+  // The value with this index, counted by the caller, ends a run.
+  __device__ __forceinline__ static bool ends(int i) {
+    return i == FIRST_RUN - 1 || i % RUN == RUN - 1;
   }
 };
 
@@ -271,9 +297,9 @@ __device__ __forceinline__ void join_moments(Moments<V>& t, int count,
   const float n = (float)count;
   float* red1 = reinterpret_cast<float*>(red);
   float a[V];
-  if (count) t.close(n);
+  t.join();
 #pragma unroll
-  for (int j = 0; j < V; ++j) a[j] = n * t.s1[j];
+  for (int j = 0; j < V; ++j) a[j] = n * t.mean[j];
   if (pl.on) put_units<V>(red1, units, a);
   __syncthreads();
   sum_groups(red1, pl, width, first, upg,
@@ -282,8 +308,8 @@ __device__ __forceinline__ void join_moments(Moments<V>& t, int count,
   if (pl.on) {
     float2 q[V];
     each_group<V>(c0 + pl.col * V, cg, [&](int j, int g) {
-      const float e = t.s1[j] - mean[g];
-      q[j] = make_float2(n * e, fmaf(n * e, e, t.s2[j]));
+      const float e = t.mean[j] - mean[g];
+      q[j] = make_float2(n * e, fmaf(n * e, e, t.m2[j]));
     });
     if (count == 0) {
 #pragma unroll
@@ -596,6 +622,7 @@ __global__ __launch_bounds__(THREADS, 4) void gn_tile(
       unpack<T, V>(raw, v);
       if (i == 0) t.about(v);
       t.add(v);
+      if (t.ends(i)) t.join();
     });
   }
   const float n = (float)s.hw * (float)s.cg;
@@ -761,10 +788,10 @@ __global__ __launch_bounds__(THREADS, 4) void gn_stats(
   for (int c0 = 0; c0 < s.c; c0 += THREADS * V) {
     const Place pl(min(THREADS, (s.c - c0) / V), THREADS);
     const int64_t next = (int64_t)pl.rows * s.c;
-    int count = 0;
+    int count = 0, batch = 0;
     Moments<V> t;
     t.begin();
-    for (int k = split; k < deal.batches; k += deal.n) {
+    for (int k = split; k < deal.batches; k += deal.n, ++batch) {
       const int here = pl.count(deal.length(k));
       const T* at = base + ((int64_t)k * deal.batch + pl.row) * s.c + c0 +
                     pl.col * V;
@@ -773,9 +800,10 @@ __global__ __launch_bounds__(THREADS, 4) void gn_stats(
       }, [&](int i, const Pack<T, V>& raw) {
         float v[V];
         unpack<T, V>(raw, v);
-        if (i == 0 && k == split) t.about(v);
+        if (i == 0 && batch == 0) t.about(v);
         t.add(v);
       });
+      if (t.ends(batch * D + D - 1)) t.join();
       count += here;
     }
     const int last = c0 + pl.cols * V;

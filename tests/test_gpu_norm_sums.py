@@ -1,0 +1,76 @@
+"""Group norm's sums where they are long: many values per thread, outliers in
+front of them.  Against sums in 64 bits.
+
+Tolerances are those of the other group norm tests: half a step of what is
+stored, and 256 steps of 2^-24 of the largest magnitude in the chain.  Sums
+keep to that at any length because none is one chain: a thread's values are
+added up in runs of at most 64, which are joined; at the sizes here that is
+below 64 + 8192 / 64 additions, and 40 more over a block and over blocks.
+"""
+
+import pytest
+import torch
+
+from deepof_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+LAST = torch.channels_last
+CHAIN = 256 * 2.0**-24
+
+
+def assert_close(got, want, magnitude):
+    assert not torch.isnan(got).any()
+    half = torch.finfo(got.dtype).eps / 2
+    off = (got.double() - want).abs() - (
+        half * want.abs() + CHAIN * (magnitude + want.abs()))
+    assert float(off.max()) <= 0, f"over the bound by {float(off.max()):.3g}"
+
+
+def normalise(x, groups, eps=1e-5):
+    """Group norm in 64 bits where x is, and the largest |xhat|."""
+    b, c, h, w = x.shape
+    v = x.double().permute(0, 2, 3, 1).reshape(b, h * w, groups, c // groups)
+    mean = v.mean((1, 3), keepdim=True)
+    v = v - mean
+    rstd = 1 / torch.sqrt(v.square().mean((1, 3), keepdim=True) + eps)
+    v = v * rstd
+    largest = float(v.abs().max() + (mean.abs() * rstd).max())
+    return v.reshape(b, h, w, c).permute(0, 3, 1, 2), largest
+
+
+LONG = [  # b, c, h, w, groups
+    (1, 1, 120, 150, 1),       # a tile, 36 values a thread
+    (1, 33, 1500, 2000, 3),    # single channels are moved, 782 values
+    (1, 36, 1500, 2000, 4),    # 4 at a time, 209
+    (1, 64, 1800, 2900, 2),    # 8 at a time, 319
+    (600, 16, 512, 160, 2),    # a block per sample, 320
+]
+
+
+@pytest.mark.parametrize("kind", ["pixel", "rows", "pixel of zeros"])
+@pytest.mark.parametrize("shape", LONG, ids=["x".join(map(str, s)) for s in LONG])
+def test_statistics_behind_outliers(shape, kind):
+    """The first values that threads meet lie far from all others: sums about
+    them are of nearly equal numbers, and round the same way again and again."""
+    b, c, h, w, groups = shape
+    g = torch.Generator(device=DEV).manual_seed(c)
+    x = torch.empty(b, h, w, c, device=DEV)
+    for i in range(b):
+        x[i].normal_(generator=g)
+    x = x.permute(0, 3, 1, 2)
+    if kind == "pixel":
+        x[:, :, 0, 0] = 3e4
+    elif kind == "rows":  # bright rows above darkness
+        rows = max(1, 20000 // w)
+        x[:, :, rows:] = 0.0
+        x[:, :, :rows] += 30
+    else:
+        x.zero_()
+        x[:, :, 0, 0] = 17.3
+    step = max(1, 200_000_000 // (c * h * w))  # samples compared at once
+    y = ops.group_norm(x, groups)
+    for i in range(0, b, step):
+        want, largest = normalise(x[i:i + step], groups)
+        assert_close(y[i:i + step], want, largest)
