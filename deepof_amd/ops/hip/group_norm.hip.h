@@ -72,6 +72,10 @@ struct Deal {
   __device__ __forceinline__ int length(int k) const {  // of batch k
     return batch - (k == batches - 1 ? missing : 0);
   }
+  // whether a block has more than `most` batches
+  __host__ __device__ __forceinline__ bool more_than(int most) const {
+    return batches > (int64_t)n * most;
+  }
 };
 
 // v + v of another lane: DPP moves within 16 lanes and between them, without
@@ -964,7 +968,9 @@ __global__ __launch_bounds__(BLOCK) void gn_apply(
 // Block (split, sample): sums of gz and gz xhat of every channel over the
 // split's pixels.  part_c: [2][b * splits][c]; part_g: [b][g][splits] of the
 // same sums weighted by w and added up over the group, which the sample's last
-// block joins.  chan, where dx is asked for: [4][b][c], for every channel its
+// block joins.  Sums are held to runs of RUN values, which are then added to a
+// thread's totals in LDS: in one chain roundings that go one way add up, and
+// 8192 equal gradients had db wrong by 6e-5.  chan, where dx is asked for: [4][b][c], for every channel its
 // mean, rstd w, and what dx adds to rstd w gz: chan2 + (x - mean) chan3.
 template <typename T, int V, int ACT, bool DROP>
 __global__ __launch_bounds__(THREADS, 4) void gn_bwd_sums(
@@ -974,12 +980,15 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_sums(
     uint64_t* __restrict__ part_g, uint32_t* __restrict__ counts,
     float* __restrict__ chan, Shape s, Deal deal, int lanes, int act,
     DropoutArgs d) {
-  extern __shared__ float lds_sums[];  // red; [2][channels]; [2][g]
+  extern __shared__ float lds_sums[];  // red; [2][channels]; [2][g]; totals
   float* red = lds_sums;
   float* sum1 = red + RED_CHANNELS(V);
   float* sum2 = sum1 + min(THREADS * V, s.c);
   float* joined = sum2 + min(THREADS * V, s.c);
   int* flag = reinterpret_cast<int*>(joined + 2 * s.g);
+  constexpr int RUN_BATCHES = RUN / AHEAD2<T>;
+  const bool runs = deal.more_than(RUN_BATCHES);
+  float* total = joined + 2 * s.g + 1 + threadIdx.x;  // [2 V][THREADS], if runs
   const int split = blockIdx.x % deal.n, b = blockIdx.x / deal.n;
   const DropoutState st = dropout_state(d);
   const float* mean = stat + (int64_t)b * s.g;
@@ -998,7 +1007,8 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_sums(
       Affine<V> k;
       k.params(ch, w, bias);
       k.stats(ch, s.cg, mean, rstd);
-      for (int kb = split; kb < deal.batches; kb += deal.n) {
+      int batch = 0;
+      for (int kb = split; kb < deal.batches; kb += deal.n, ++batch) {
         const int here = pl.count(deal.length(kb));
         const int64_t at = ((int64_t)b * s.hw + (int64_t)kb * deal.batch +
                             pl.row) * s.c + ch;
@@ -1015,6 +1025,22 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_sums(
             s2[j] = fmaf(g[j], e[j], s2[j]);
           }
         });
+        if (runs && batch % RUN_BATCHES == RUN_BATCHES - 1) {
+#pragma unroll
+          for (int j = 0; j < 2 * V; ++j) {
+            float* at = total + j * THREADS;
+            float& sum = j < V ? s1[j % V] : s2[j % V];
+            *at = batch < RUN_BATCHES ? sum : *at + sum;
+            sum = 0.0f;
+          }
+        }
+      }
+      if (runs) {  // every block has had one
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          s1[j] += total[j * THREADS];
+          s2[j] += total[(V + j) * THREADS];
+        }
       }
       each_group<V>(ch, s.cg, [&](int j, int g) { s2[j] *= rstd[g]; });
     }
@@ -1386,8 +1412,10 @@ void gn_backward(const at::Tensor& x, const at::Tensor& gy, at::Tensor& dx_out,
   const bool nt = x.numel() * (int64_t)sizeof(T) > STREAM_BYTES;
   GN_VARIANT(v, act, d.on, {
     auto sums = gn_bwd_sums<T, V, ACT, DROP>;
-    const size_t lds = 4 * (RED_CHANNELS(V) + 2 * s.g + 1 +
-                            2 * (size_t)std::min(THREADS * V, s.c));
+    const size_t lds =
+        4 * (RED_CHANNELS(V) + 2 * s.g + 1 +
+             2 * (size_t)std::min(THREADS * V, s.c) +
+             (deal.more_than(RUN / AHEAD2<T>) ? 2 * V * THREADS : 0));
     allow_lds(sums, lds);
     hipLaunchKernelGGL(sums, dim3(s.b * deal.n), dim3(THREADS), lds, stream, px,
                        pg, w, bias, stat, part_c, part_g, counts,

@@ -74,3 +74,19 @@ def test_statistics_behind_outliers(shape, kind):
     for i in range(0, b, step):
         want, largest = normalise(x[i:i + step], groups)
         assert_close(y[i:i + step], want, largest)
+
+
+def test_gradient_sums_of_many_values():
+    """8192 values a thread.  What a mean hands back is the same everywhere."""
+    b, c, h, w = 1, 511, 1448, 1448
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.empty(b, h, w, c, device=DEV)
+    x.normal_(generator=g)
+    x = x.permute(0, 3, 1, 2)
+    bias = torch.zeros(c, device=DEV, requires_grad=True)
+    gy = torch.full_like(x, 0.1)
+    y = ops.group_norm(x, 7, None, bias)
+    db = torch.autograd.grad(y, bias, gy)[0]
+    want = torch.full((c,), float(gy[0, 0, 0, 0].double()) * h * w,
+                      device=DEV, dtype=torch.float64)
+    assert_close(db, want, float(want[0]))
