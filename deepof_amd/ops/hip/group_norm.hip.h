@@ -158,6 +158,14 @@ __device__ __forceinline__ void add_to(float2& a, float2 b) {
   a.x += b.x;
   a.y += b.y;
 }
+// One of many additions, as many as there are samples: what its rounding loses
+// goes into the next (Kahan's sum).
+__device__ __forceinline__ void add_kept(float& sum, float& lost, float v) {
+  v -= lost;
+  const float next = sum + v;
+  lost = (next - sum) - v;
+  sum = next;
+}
 __device__ __forceinline__ float over_wave(float v) { return wave_sum(v); }
 __device__ __forceinline__ float2 over_wave(float2 v) {
   return make_float2(wave_sum(v.x), wave_sum(v.y));
@@ -591,6 +599,10 @@ struct Tiles {
   int iters;        // vectors per thread
 };
 
+// Threads of a channel that share its samples in a span's last block.
+__host__ __device__ __forceinline__ int sample_shares(int span) {
+  return THREADS > span ? THREADS / span : 1;
+}
 
 // LDS: the tile, red, then floats per group.
 template <typename T, int V, int ACT, bool DROP>
@@ -658,6 +670,7 @@ __global__ __launch_bounds__(THREADS, 4) void gn_tile(
 // LDS: x's and gy's tiles, red, then floats per channel and per group.
 // sums_c: [b][c] of the samples' sums of gz and gz xhat, which the last block
 // of a span adds up to the parameters' gradients; null: none is asked for.
+// counts null: they are left as [2][b][c] for gn_param_grad.
 template <typename T, int V, int ACT, bool DROP>
 __global__ __launch_bounds__(THREADS, 4) void gn_bwd_tile(
     const T* __restrict__ x, const T* __restrict__ gy, T* __restrict__ dx,
@@ -719,9 +732,18 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_tile(
                  t1[g - span * tiles.groups] = -r * (a * inv_n);
                  t2[g - span * tiles.groups] = -r * r * (c * inv_n);
                });
-  if (sums_c)
-    for (int c = threadIdx.x; c < tiles.span; c += THREADS)
-      put2(sums_c + (int64_t)b * s.c + c0 + c, sum1[c], sum2[c]);
+  if (sums_c) {
+    const int64_t at = (int64_t)b * s.c + c0;
+    float* part = reinterpret_cast<float*>(sums_c) + at;
+    for (int c = threadIdx.x; c < tiles.span; c += THREADS) {
+      if (counts) {
+        put2(sums_c + at + c, sum1[c], sum2[c]);
+      } else {
+        part[c] = sum1[c];
+        part[(int64_t)s.b * s.c + c] = sum2[c];
+      }
+    }
+  }
   __syncthreads();
   if (dx && count) {
     float m1[V], m2[V];
@@ -741,20 +763,30 @@ __global__ __launch_bounds__(THREADS, 4) void gn_bwd_tile(
       store_pack<T, V>(dx + at, pack<T, V>(g));
     }
   }
-  if (!sums_c || !last_of(s.b, counts + span, flag)) return;
+  if (!sums_c || !counts || !last_of(s.b, counts + span, flag)) return;
   // samples dealt in `shares` to threads that lie a span apart
-  const int shares = max(1, small_div(THREADS, tiles.span));
+  const int shares = sample_shares(tiles.span);
   const int share = shares > 1 ? small_div(threadIdx.x, tiles.span) : 0;
   float2* red2 = reinterpret_cast<float2*>(red);
   for (int c1 = 0; c1 < tiles.span; c1 += THREADS) {
     const int c = c1 + threadIdx.x - share * tiles.span;
     const bool in = c < tiles.span && share < shares;
-    float2 sum = make_float2(0.0f, 0.0f);
+    float2 sum = make_float2(0.0f, 0.0f), lost = sum;
     if (in) {
       const uint64_t* at = sums_c + c0 + c;
-#pragma unroll 8
-      for (int i = share; i < s.b; i += shares)
-        add_to(sum, get2(at + (int64_t)i * s.c));
+      constexpr int D = 8;  // asked for at once
+      for (int i = share; i < s.b; i += D * shares) {
+        float2 v[D];
+#pragma unroll
+        for (int q = 0; q < D; ++q)
+          v[q] = get2(at + (int64_t)min(i + q * shares, s.b - 1) * s.c);
+#pragma unroll
+        for (int q = 0; q < D; ++q) {
+          if (i + q * shares >= s.b) v[q] = make_float2(0.0f, 0.0f);
+          add_kept(sum.x, lost.x, v[q].x);
+          add_kept(sum.y, lost.y, v[q].y);
+        }
+      }
     }
     red2[threadIdx.x] = sum;
     __syncthreads();
@@ -1106,10 +1138,11 @@ __device__ __forceinline__ void param_sums(const float* __restrict__ part,
     float* out = which ? dw : db;
     if (!out) continue;
     const float* at = part + (int64_t)which * rows * c + ch;
-    float sum = 0.0f;
+    float sum = 0.0f, lost = 0.0f;
     if (ch < c) {
 #pragma unroll 8
-      for (int64_t r = r0; r < rows; r += BLOCK / 8) sum += at[r * c];
+      for (int64_t r = r0; r < rows; r += BLOCK / 8)
+        add_kept(sum, lost, at[r * c]);
     }
     red[threadIdx.x] = sum;
     __syncthreads();
@@ -1244,6 +1277,14 @@ Plan plan_tiles(const Shape& s, int v, size_t value, bool back) {
   }
   return p;
 }
+
+// Samples that a thread of a span's last block adds up, at most: of more,
+// another launch takes the sums, with more than one block's share of the
+// memory's rate.  Backward passes, bf16, in us: 4096x64x4x4, 512 samples a
+// thread, 92 here and 57 there; one pixel of 512 channels, 1024 samples 78 and
+// 55, 4096 samples 281 and 71.  512 of those, where the host's part is longer
+// than the kernels, take 53 and 57.
+constexpr int64_t MOST_SAMPLES = 256;
 
 int join_blocks(const Shape& s, int lanes) {
   const int groups = THREADS / lanes;
@@ -1391,6 +1432,8 @@ void gn_backward(const at::Tensor& x, const at::Tensor& gy, at::Tensor& dx_out,
       sums = (uint64_t*)buf.data_ptr();
     }
     const float* rstd = stat + (int64_t)s.b * s.g;
+    const bool many = s.b > MOST_SAMPLES * sample_shares(p.tiles.span);
+    if (many) counts = nullptr;
     GN_VARIANT(v, act, d.on, {
       auto kernel = gn_bwd_tile<T, V, ACT, DROP>;
       allow_lds(kernel, p.lds);
@@ -1399,6 +1442,11 @@ void gn_backward(const at::Tensor& x, const at::Tensor& gy, at::Tensor& dx_out,
                          counts, db, dw, s, p.tiles, act, d);
       C10_HIP_KERNEL_LAUNCH_CHECK();
     });
+    if (sums && many) {
+      hipLaunchKernelGGL(gn_param_grad, dim3((s.c + 7) / 8), dim3(BLOCK), 0,
+                         stream, (const float*)sums, (int64_t)s.b, s.c, db, dw);
+      C10_HIP_KERNEL_LAUNCH_CHECK();
+    }
     return;
   }
   const int param_blocks = db || dw ? (s.c + 7) / 8 : 0;

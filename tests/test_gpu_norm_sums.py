@@ -1,11 +1,12 @@
 """Group norm's sums where they are long: many values per thread, outliers in
-front of them.  Against sums in 64 bits.
+front of them, many samples.  Against sums in 64 bits.
 
 Tolerances are those of the other group norm tests: half a step of what is
 stored, and 256 steps of 2^-24 of the largest magnitude in the chain.  Sums
 keep to that at any length because none is one chain: a thread's values are
-added up in runs of at most 64, which are joined; at the sizes here that is
-below 64 + 8192 / 64 additions, and 40 more over a block and over blocks.
+added up in runs of at most 64, which are joined, below 64 + 8192 / 64 additions
+at the sizes here, 40 more over a block and over blocks, and 64 where shares of
+the samples meet; a share's own sum carries along what its roundings lose.
 """
 
 import pytest
@@ -90,3 +91,22 @@ def test_gradient_sums_of_many_values():
     want = torch.full((c,), float(gy[0, 0, 0, 0].double()) * h * w,
                       device=DEV, dtype=torch.float64)
     assert_close(db, want, float(want[0]))
+
+
+@pytest.mark.parametrize("shape", [(100_000, 512, 1, 1, 32),
+                                   (4096, 8, 3, 3, 2), (2048, 515, 2, 2, 5)])
+def test_parameter_gradients_over_many_samples(shape):
+    b, c, h, w, groups = shape
+    g = torch.Generator(device=DEV).manual_seed(6)
+    x = torch.randn(b, h, w, c, device=DEV, generator=g).permute(0, 3, 1, 2)
+    weight = torch.ones(c, device=DEV, requires_grad=True)
+    bias = torch.zeros(c, device=DEV, requires_grad=True)
+    gy = torch.full_like(x, 0.1)
+    y = ops.group_norm(x, groups, weight, bias)
+    dw, db = torch.autograd.grad(y, (weight, bias), gy)
+    step = float(gy[0, 0, 0, 0].double())
+    n = b * h * w
+    want = torch.full((c,), step * n, device=DEV, dtype=torch.float64)
+    assert_close(db, want, step * n)
+    xhat, largest = normalise(x, groups)
+    assert_close(dw, step * xhat.sum((0, 2, 3)), step * n * (1 + largest))
