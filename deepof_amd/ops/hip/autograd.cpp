@@ -139,11 +139,18 @@ void check_values(const Tensor& x, const char* name) {
                    x.scalar_type());
 }
 
+// A tangent would be lost: kernels read a dual tensor's value alone.
+void no_tangent(const Tensor& t, const char* name) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name,
+                              ": no forward-mode derivatives on the GPU");
+}
+
 // A parameter as the kernels read it: fp32, contiguous.  A cast is part of the
 // graph.
 OptTensor param(const OptTensor& t, const Tensor& x, const char* name) {
   if (!t.has_value() || !t->defined()) return c10::nullopt;
   check_values(*t, name);
+  no_tangent(*t, name);
   TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == x.size(1) &&
                         t->device() == x.device(),
                     name, " must be [", x.size(1), "] on ", x.device(),
@@ -158,6 +165,7 @@ Tensor group_norm(const Tensor& input, int64_t groups, const OptTensor& weight,
                   const OptTensor& bias, double eps, int64_t act, double p,
                   const OptTensor& rng, int64_t seed, int64_t offset) {
   check_values(input, "group_norm");
+  no_tangent(input, "group_norm");
   TORCH_CHECK_VALUE(input.dim() == 4, "group_norm: [B, C, H, W] expected, got ",
                     input.sizes());
   const int64_t c = input.size(1);
@@ -184,6 +192,7 @@ Tensor group_norm(const Tensor& input, int64_t groups, const OptTensor& weight,
 Tensor dropout(const Tensor& input, int64_t act, double p, const OptTensor& rng,
                int64_t seed, int64_t offset) {
   check_values(input, "dropout");
+  no_tangent(input, "dropout");
   const Tensor x = input.contiguous(dense_format(input));
   if (at::GradMode::is_enabled() && x.requires_grad())
     return Dropout::apply(x, act, p, rng, seed, offset);
