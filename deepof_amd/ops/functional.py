@@ -313,7 +313,8 @@ def dropout(x: torch.Tensor, p: float = 0.5, rng=None,
     p is held to 2^-32.  A captured graph replays the mask of a pair of ints;
     it reads a tensor anew, and draws anew where rng is None.
 
-    On the GPU forward-mode derivatives raise NotImplementedError.
+    On the GPU forward-mode derivatives and tracing (torch.jit.trace, make_fx)
+    raise NotImplementedError.
     """
     code = _act_code(act)
     if not isinstance(x, torch.Tensor):
@@ -338,7 +339,8 @@ def group_norm(x: torch.Tensor, num_groups: int,
     "elu", "leaky_relu" (0.1), "relu" or "silu".  dropout: its probability;
     rng as for `dropout`, whose mask for the same rng is the same.
 
-    On the GPU forward-mode derivatives raise NotImplementedError.
+    On the GPU forward-mode derivatives and tracing (torch.jit.trace, make_fx)
+    raise NotImplementedError.
     """
     code = _act_code(act)
     if not isinstance(x, torch.Tensor):

@@ -2,7 +2,9 @@
 // Python function's backward would take the interpreter's lock from the
 // engine's thread, some 20 us that small activations feel.
 
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -145,6 +147,16 @@ void no_tangent(const Tensor& t, const char* name) {
                               ": no forward-mode derivatives on the GPU");
 }
 
+// A tracer would record the result's allocation and not the kernels.
+void not_traced(const char* name) {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !torch::jit::tracer::isTracing() &&
+          !TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY),
+      name, ": cannot be traced on the GPU");
+}
+
 // A parameter as the kernels read it: fp32, contiguous.  A cast is part of the
 // graph.
 OptTensor param(const OptTensor& t, const Tensor& x, const char* name) {
@@ -164,6 +176,7 @@ OptTensor param(const OptTensor& t, const Tensor& x, const char* name) {
 Tensor group_norm(const Tensor& input, int64_t groups, const OptTensor& weight,
                   const OptTensor& bias, double eps, int64_t act, double p,
                   const OptTensor& rng, int64_t seed, int64_t offset) {
+  not_traced("group_norm");
   check_values(input, "group_norm");
   no_tangent(input, "group_norm");
   TORCH_CHECK_VALUE(input.dim() == 4, "group_norm: [B, C, H, W] expected, got ",
@@ -191,6 +204,7 @@ Tensor group_norm(const Tensor& input, int64_t groups, const OptTensor& weight,
 
 Tensor dropout(const Tensor& input, int64_t act, double p, const OptTensor& rng,
                int64_t seed, int64_t offset) {
+  not_traced("dropout");
   check_values(input, "dropout");
   no_tangent(input, "dropout");
   const Tensor x = input.contiguous(dense_format(input));

@@ -36,3 +36,15 @@ def test_forward_mode_derivatives_of_parameters_are_refused(which):
         p[which] = fwd.make_dual(p[which], torch.ones(4, device=DEV))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             ops.group_norm(x, 2, **p)
+
+
+@pytest.mark.parametrize("call", CALLS.values(), ids=CALLS)
+def test_tracing_is_refused(call):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = torch.randn(1, 4, 3, 3, device=DEV)
+    with pytest.raises(NotImplementedError, match="cannot be traced"):
+        torch.jit.trace(call, x)
+    with pytest.raises(NotImplementedError, match="cannot be traced"):
+        make_fx(call)(x)
+    call(x)
