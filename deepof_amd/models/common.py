@@ -34,17 +34,15 @@ def check_norm(norm: str | None) -> None:
 
 def _with_norm(build, cout: int, act: str | None, norm: str | None,
                dropout: float) -> nn.Module:
-    """build(act) with a group norm between it and its activation, and dropout
-    behind that."""
-    from ..ops.norm import CounterDropout, GroupNormAct
+    """build(act, dropout) with a group norm between it and its activation,
+    and dropout behind that."""
+    from ..ops.norm import GroupNormAct
 
     check_norm(norm)
     if norm == "group":
-        return nn.Sequential(build(None), GroupNormAct(cout, act,
-                                                       dropout=dropout))
-    if dropout:
-        return nn.Sequential(build(None), CounterDropout(dropout, act))
-    return build(act)
+        return nn.Sequential(build(None, 0.0), GroupNormAct(cout, act,
+                                                            dropout=dropout))
+    return build(act, dropout)
 
 
 def act_dropout(act: str, p: float, rng: str) -> list[nn.Module]:
@@ -64,8 +62,8 @@ def conv(cin: int, cout: int, k: int = 3, stride: int = 1,
          dropout: float = 0.0) -> nn.Module:
     from ..ops.conv import FusedConvAct
 
-    return _with_norm(lambda a: FusedConvAct(cin, cout, k, stride, a), cout,
-                      act, norm, dropout)
+    return _with_norm(lambda a, p: FusedConvAct(cin, cout, k, stride, a, p),
+                      cout, act, norm, dropout)
 
 
 def deconv(cin: int, cout: int, act: str | None = "elu",
@@ -77,8 +75,8 @@ def deconv(cin: int, cout: int, act: str | None = "elu",
     nn.ConvTranspose2d."""
     from ..ops.deconv import FusedDeconvAct
 
-    return _with_norm(lambda a: FusedDeconvAct(cin, cout, a), cout, act, norm,
-                      dropout)
+    return _with_norm(lambda a, p: FusedDeconvAct(cin, cout, a, p), cout, act,
+                      norm, dropout)
 
 
 def bilinear_deconv_weight(cin: int, cout: int, k: int = 4) -> torch.Tensor:

@@ -18,6 +18,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .norm import CounterDropout
+
 _ACT_CODE = {None: 0, "none": 0, "elu": 1, "leaky_relu": 2, "relu": 3}
 _CODE_ACT = {0: "none", 1: "elu", 2: "leaky_relu", 3: "relu"}
 _dispatch_cache: dict[tuple, str] = {}
@@ -133,15 +135,40 @@ def _conv_backward_impl(ctx, gy):
     return gx, gw, gb, None, None, None
 
 
-class FusedConvAct(nn.Module):
-    """Conv2d + bias + activation; HIP MFMA kernel on GPU when it wins."""
+class FusedAct(nn.Module):
+    """A layer with an activation, and dropout behind it on request, which
+    then takes the activation into its own pass.
 
-    def __init__(self, cin, cout, k=3, stride=1, act: str | None = "elu"):
+    Dropout has no parameters: a state_dict with it fits a layer without, and
+    the other way round.
+    """
+
+    def __init__(self, act: str | None, dropout: float):
         super().__init__()
+        self.drop = CounterDropout(dropout, act) if dropout else None
+        self.act_name = None if dropout else act
+        self.act_code = _ACT_CODE[self.act_name]
+
+    def forward(self, x):
+        y = self._layer(x)
+        return y if self.drop is None else self.drop(y)
+
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        # layers with dropout were the first of two modules once
+        for key in [k for k in state_dict if k.startswith(prefix + "0.")]:
+            state_dict[prefix + key[len(prefix) + 2:]] = state_dict.pop(key)
+        super()._load_from_state_dict(state_dict, prefix, *args)
+
+
+class FusedConvAct(FusedAct):
+    """Conv2d + bias + activation (+ dropout); HIP MFMA kernel on GPU when it
+    wins."""
+
+    def __init__(self, cin, cout, k=3, stride=1, act: str | None = "elu",
+                 dropout: float = 0.0):
+        super().__init__(act, dropout)
         self.conv = nn.Conv2d(cin, cout, k, stride=stride, padding=k // 2,
                               bias=True)
-        self.act_name = act
-        self.act_code = _ACT_CODE[act]
         self.cin, self.k, self.stride = cin, k, stride
 
     def _hip_eligible(self, x):
@@ -181,7 +208,7 @@ class FusedConvAct(nn.Module):
         return _MiopenConvFn.apply(x, w, self.conv.bias, self.stride,
                                    self.k // 2, self.act_code)
 
-    def forward(self, x):
+    def _layer(self, x):
         if not self._hip_eligible(x):
             return self._miopen(x)
         key = (self.cin, self.conv.out_channels, self.k, self.stride,

@@ -24,6 +24,8 @@ import time
 
 import torch
 
+from .conv import FusedAct
+
 _EMPTY = None
 
 
@@ -186,8 +188,8 @@ class _FusedDeconvFn(torch.autograd.Function):
 _deconv_cache: dict[tuple, str] = {}
 
 
-class FusedDeconvAct(torch.nn.Module):
-    """4x4/s2 transposed conv + bias + activation.
+class FusedDeconvAct(FusedAct):
+    """4x4/s2 transposed conv + bias + activation (+ dropout).
 
     GPU: sub-pixel MFMA kernel (4 parity launches, fused bias+act) when
     it measures faster than MIOpen for the shape; params live in a
@@ -195,14 +197,11 @@ class FusedDeconvAct(torch.nn.Module):
     starts are unchanged.
     """
 
-    def __init__(self, cin: int, cout: int, act: str | None = "elu"):
-        super().__init__()
-        from .conv import _ACT_CODE
-
+    def __init__(self, cin: int, cout: int, act: str | None = "elu",
+                 dropout: float = 0.0):
+        super().__init__(act, dropout)
         self.deconv = torch.nn.ConvTranspose2d(cin, cout, 4, stride=2,
                                                padding=1, bias=True)
-        self.act_name = act
-        self.act_code = _ACT_CODE[act]
         self.cin, self.cout = cin, cout
 
     def _torch(self, x):
@@ -220,7 +219,7 @@ class FusedDeconvAct(torch.nn.Module):
         x = x.contiguous(memory_format=torch.channels_last)
         return _FusedDeconvFn.apply(x, w, self.deconv.bias, self.act_code)
 
-    def forward(self, x):
+    def _layer(self, x):
         import os
 
         if os.environ.get("DEEPOF_NO_DECONV"):
