@@ -48,10 +48,17 @@ MODEL_REGISTRY = {
 
 def norm_kwargs(cfg) -> dict:
     """What a config says of normalisation and dropout, as arguments of its
-    model; a model's parameters depend on the first of them."""
+    model; a model's parameters depend on the first of them.
+
+    ValueError where a classifier's dropout is configured and the model has
+    no classifier."""
     kwargs = {"norm": cfg.norm, "feature_dropout": cfg.feature_dropout}
     if cfg.model in ("st_single", "st_baseline"):
         kwargs["dropout_rng"] = cfg.dropout_rng
+    elif cfg.dropout_rng != "torch":
+        raise ValueError(f"dropout_rng={cfg.dropout_rng!r}: {cfg.model} has no "
+                         "classifier with dropout (feature_dropout has no "
+                         "other generator)")
     return kwargs
 
 
