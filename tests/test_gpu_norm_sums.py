@@ -110,3 +110,54 @@ def test_parameter_gradients_over_many_samples(shape):
     assert_close(db, want, step * n)
     xhat, largest = normalise(x, groups)
     assert_close(dw, step * xhat.sum((0, 2, 3)), step * n * (1 + largest))
+
+
+@pytest.mark.parametrize("shape", [
+    (1, 33, 1500, 2000, 3), (1, 36, 1500, 2000, 4), (1, 64, 1800, 2900, 2),
+    (1, 4096, 132, 131, 4096),  # as much of LDS as there may be
+], ids=lambda s: "x".join(map(str, s)))
+def test_gradients_of_long_threads(shape):
+    b, c, h, w, groups = shape
+    g = torch.Generator(device=DEV).manual_seed(7)
+    x, gy = (torch.randn(b, h, w, c, device=DEV, generator=g)
+             .permute(0, 3, 1, 2) for _ in range(2))
+    weight = 1 + 0.3 * torch.randn(c, device=DEV, generator=g)
+    leaves = [t.requires_grad_() for t in
+              (x, weight, torch.zeros(c, device=DEV))]
+    y = ops.group_norm(x, groups, *leaves[1:])
+    dx, dw, db = torch.autograd.grad(y, leaves, gy)
+    del y
+    x, weight = x.detach(), weight.detach()
+    xhat, largest = normalise(x, groups)
+    gz = gy.double()
+    total = float(gz.abs().sum((0, 2, 3)).max())
+    assert_close(db, gz.sum((0, 2, 3)), total)
+    assert_close(dw, (gz * xhat).sum((0, 2, 3)), total * (1 + largest))
+    gz *= weight.double().view(1, -1, 1, 1)
+    top = float(gz.abs().max())
+
+    def over_groups(t):  # the mean of each value's group
+        v = t.reshape(b, groups, -1).mean(2)
+        return v.repeat_interleave(c // groups, 1).view(b, c, 1, 1)
+
+    var = over_groups((x.double() - over_groups(x.double())).square())
+    rstd = 1 / torch.sqrt(var + 1e-5)
+    want = rstd * (gz - over_groups(gz) - xhat * over_groups(gz * xhat))
+    assert_close(dx, want, float(rstd.max()) * top * (2 + largest) ** 2)
+
+
+def test_statistics_behind_2_31_elements():
+    """The last sample, whose every element lies behind 2^31: 1056 values a
+    thread, against sums in 64 bits."""
+    b, c, h, w, groups = 3, 64, 3400, 3400, 8
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.empty(b, h, w, c, dtype=torch.bfloat16, device=DEV)
+    for i in range(b):
+        x[i].normal_(generator=g)
+    x = x.permute(0, 3, 1, 2)
+    assert x.numel() > 2**31
+    y = ops.group_norm(x, groups)
+    for group in (0, groups - 1):
+        at = slice(group * c // groups, (group + 1) * c // groups)
+        want, largest = normalise(x[-1:, at], 1)
+        assert_close(y[-1:, at], want, largest)
