@@ -24,10 +24,11 @@
 //    last launch reads x (and gy) again: three launches forwards (sums, their
 //    join, y), two backwards (sums, whose last blocks join them; dx).
 // 64x64x192x256 bf16 with ELU (403 MB a tensor; 1.6 GB is the least that
-// forward and backward move, 3.2 GB is what the split route does): sums 119 us,
-// join 5, y 118; sums 196, dx 182: 5.2 TB/s over all, what a large copy reaches
-// here.  8x24x32x512 bf16 (tile; 6.3 MB): 9.7 us forwards, 13.2 backwards, most
-// of it launch, first loads and the sums' three meetings in LDS.
+// forward and backward move, 3.2 GB is what the split route does): sums 118 us,
+// join 5, y 117; sums 194, dx 183: 5.2 TB/s over all, what a large copy reaches
+// here, the sums below it and the others above.  8x24x32x512 bf16 (tile; 6.3
+// MB): 9.8 us forwards, 13.3 backwards, most of it launch, first loads and the
+// sums' three meetings in LDS.
 // Keeping larger samples on the chip, a team of blocks each with its tile, was
 // built and measured too: a team's meeting costs its blocks some 20 us, in
 // which a CU's LDS holds far less than memory moves, and 64x64x192x256 bf16
@@ -60,9 +61,10 @@ using Shape = GroupNormShape;
 
 // A sample's pixels dealt to n blocks: batches of `batch` pixels, of which
 // block i takes i, i + n, ...  Blocks that run together then read neighbouring
-// memory.  (Each with a long piece of its own, whose lengths are large powers
-// of 2 here, they met at the same memory channels: 403 MB took 113 us to read,
-// not 70.)
+// memory.  Forward sums of 403 MB take 109 us behind kernels that only read and
+// 118 behind one that wrote; with a long piece per block they took 113.  Reading
+// alone takes 62 to 71: a wave asks for its next batch only once it has summed
+// the one before, which is the likely reason for the rest.
 struct Deal {
   int n, batch, batches, missing;  // missing: pixels that the last batch lacks
   __device__ __forceinline__ int pixels(int i) const {
@@ -556,6 +558,15 @@ __device__ __forceinline__ float2 get2(const uint64_t* at) {
 
 // Whether this block is the last of `blocks`.  All its threads call it; their
 // put2 calls are done before it counts.  flag: LDS.
+//
+// What orders parts and count is this machine, not the language: put2's stores
+// and get2's loads go to where all XCDs meet, every wave has waited for its
+// stores (vmcnt counts them until they are there) before the barrier behind
+// which thread 0 counts, and loads stand behind the count's return and another
+// barrier.  Counting with acquire and release at agent scope says as much, but
+// writes back and drops an L2's lines at every count: 8x24x32x512 bf16 took
+// 19.2 us backwards with it, not 13.2, and the sums of 64x64x192x256 205, not
+// 194.
 __device__ __forceinline__ bool last_of(int blocks, uint32_t* count,
                                         int* flag) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

@@ -49,7 +49,6 @@ __device__ __forceinline__ void store_pack(T* at, const Pack<T, V>& p) {
   *reinterpret_cast<Pack<T, V>*>(at) = p;
 }
 
-// ACT_ANY: not known at compile time, passed in.
 // The same past the caches, where `stream` (uniform) says that what is moved
 // is larger than they are.  403 MB are copied in 134 us so, in 148 us else;
 // what fits is better kept for who reads it next.
@@ -88,6 +87,7 @@ __device__ __forceinline__ void store_pack(T* at, const Pack<T, V>& p,
 // Bytes of a tensor above which it is streamed: the L2s' 32 MB.
 constexpr int64_t STREAM_BYTES = 32ll << 20;
 
+// ACT_ANY: not known at compile time, passed in.
 enum Act { ACT_ANY = -1, ACT_NONE = 0, ACT_ELU = 1, ACT_LEAKY = 2, ACT_RELU = 3,
            ACT_SILU = 4 };
 
