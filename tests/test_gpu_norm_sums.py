@@ -161,3 +161,54 @@ def test_statistics_behind_2_31_elements():
         at = slice(group * c // groups, (group + 1) * c // groups)
         want, largest = normalise(x[-1:, at], 1)
         assert_close(y[-1:, at], want, largest)
+
+
+@pytest.mark.parametrize("shape", [
+    (2048, 515, 2, 2, 5),     # parameters' gradients by a launch of their own
+    (2, 64, 700, 800, 8),     # totals in LDS
+], ids=lambda s: "x".join(map(str, s)))
+def test_replays_of_long_sums(shape):
+    b, c, h, w, groups = shape
+    g = torch.Generator(device=DEV).manual_seed(8)
+    x, gy = (torch.randn(b, h, w, c, device=DEV, generator=g).bfloat16()
+             .permute(0, 3, 1, 2) for _ in range(2))
+    weight, bias = (torch.randn(c, device=DEV, generator=g) for _ in range(2))
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in (x, weight, bias)]
+        y = ops.group_norm(leaves[0], groups, *leaves[1:], act="silu")
+        return [y.detach(), *torch.autograd.grad(y, leaves, gy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(4):
+        x.normal_(generator=g)
+        gy.normal_(generator=g)
+        want = step()
+        for t in out:
+            t.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, e in zip(out, want):
+            assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("at", [0, 5 * 800 + 3, -1], ids=["first", "amid", "last"])
+def test_what_is_not_finite_stays_in_its_group(bad, at):
+    """Wherever among a thread's runs it comes."""
+    x = torch.randn(600, 800, 16, device=DEV)
+    x = x.permute(2, 0, 1).unsqueeze(0)
+    clean = ops.group_norm(x, 4)
+    x.permute(0, 2, 3, 1).view(-1, 16)[at, 5] = bad
+    y = ops.group_norm(x, 4)
+    assert torch.isnan(y[:, 4:8]).all()
+    assert torch.equal(y[:, :4], clean[:, :4])
+    assert torch.equal(y[:, 8:], clean[:, 8:])
